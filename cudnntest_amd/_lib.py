@@ -16,7 +16,8 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _u = ctypes.c_uint
 _l = ctypes.c_long
-
+_ll = ctypes.c_longlong
+_sz = ctypes.c_size_t
 
 
 class StackLayer(ctypes.Structure):
@@ -60,6 +61,15 @@ SYMBOLS = {
     "wino_stage_timing": (_i, [_i]),
     "wino_stage_times": (_i, [ctypes.POINTER(ctypes.c_float), ctypes.POINTER(_l)]),
     "wino_stage_stats": (_i, [ctypes.POINTER(ctypes.c_float)] * 3 + [ctypes.POINTER(_l)]),
+    "wino_mx4_geometry": (_i, [_i, _i, _ip, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "wino_mx4_quantize": (_i, [_i] * 3 + [_vp] * 4),
+    "wino_mx4_dequantize": (_i, [_i] * 3 + [_vp] * 4),
+    "wino_mx4_workspace_bytes": (_sz, [_i] * 3),
+    "wino_mx4_gemm": (_i, [_i, _u] + [_i] * 3 + [_vp] * 7 + [_sz, _vp]),
+    "wino_mx4_linear": (_i, [_i, _u] + [_i] * 3 + [_vp] * 6 + [_sz, _vp]),
+    "wino_linear_cross_entropy_workspace_bytes": (_sz, [_i] * 4 + [_vp, _vp, _i]),
+    "wino_linear_cross_entropy": (_i, [_i] * 4 + [_vp] * 4 + [_ll] + [_vp] * 3 + [_sz, _vp]),
+    "wino_linear_cross_entropy_backward": (_i, [_i] * 4 + [_vp] * 4 + [_ll] + [_vp] * 6 + [_sz, _vp]),
     "wino_warmup": (_i, []),
     "wino_sync": (_i, [_vp]),
     "wino_last_error": (ctypes.c_char_p, []),
@@ -71,7 +81,7 @@ _lib = None
 
 def build():
     """Compile the HIP sources for gfx950 (hipcc cross-compiles without a GPU)."""
-    subprocess.check_call(["make", "-s", "-B", "-C", CSRC])
+    subprocess.check_call(["make", "-s", "-B", "-j4", "-C", CSRC])
     return LIB_PATH
 
 

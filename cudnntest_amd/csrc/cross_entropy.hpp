@@ -1,0 +1,290 @@
+// Softmax cross entropy of linear logits, and its gradient, without the logits in memory.
+//
+//   l[t][v] = sum_d x[t][d] w[v][d] + bias[v]
+//   lse[t]  = log sum_v exp l[t][v]                loss[t] = lse[t] - l[t][target[t]]   (0 for an ignored row)
+//   dl[t][v] = grad[t] * (exp(l[t][v] - lse[t]) - [v == target[t]])                     (0 for an ignored row)
+//   dx = dl w        dw = dl^T x        dbias[v] = sum_t dl[t][v]
+//
+// The products run on tile_gemm_kernel with the vocabulary on the tile's m side: a lane then holds one row t and up to
+// 64 of its logits in registers, so the softmax statistics of a tile need no exchange between lanes but one.
+// Forward: every tile leaves (max, sum of exp) per row, 8 bytes for 128 logits, and one kernel joins them.  Backward:
+// the vocabulary is taken in pieces; a piece's dl (in the tensors' type) goes to scratch and feeds the two products.
+#pragma once
+#include "common.hpp"
+#include "tile_gemm.hpp"
+
+namespace wino {
+
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// (max, sum of exp(l - max)) of the union of two sets of logits; the empty set is (-inf, 0)
+__device__ __forceinline__ void stats_join(float& mx, float& sum, float mx2, float sum2) {
+    const float m = fmaxf(mx, mx2);
+    // both empty, or both all -inf: no exp(-inf + inf).  A NaN sum stays one: fmaxf drops the NaN of a maximum.
+    const float a = mx == m ? sum : sum * exp_of(mx - m), b = mx2 == m ? sum2 : sum2 * exp_of(mx2 - m);
+    sum = a + b;
+    mx = m;
+}
+
+// a target outside the vocabulary that is not `ignore` makes its row's loss and gradient NaN
+struct CeRows {
+    const long long* target;
+    long long ignore;
+    int V;
+};
+
+// ---- epilogues ---------------------------------------------------------------------------------
+
+// stats[tile][t] = (max, sum) over the tile's logits; picked[t] = the target's logit
+template <typename T> struct CeStats {
+    const T* bias;
+    CeRows rows;
+    float2* stats;
+    float* picked;
+    template <int BM, int BN, int WM, int WN, int MI, int NI>
+    __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char* lds) const {
+        float mx[NI], sum[NI];
+#pragma unroll
+        for (int n = 0; n < NI; ++n) mx[n] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int m = m0 + (wm * MI + i) * 32 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                const float b = bias && m < g.M ? to_f32(bias[m]) : 0.f;
+#pragma unroll
+                for (int n = 0; n < NI; ++n) {
+                    const float l = m < g.M ? acc[i][n][r] + b : -INFINITY;
+                    acc[i][n][r] = l;
+                    mx[n] = fmaxf(mx[n], l);
+                }
+            }
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int t = n0 + (wn * NI + n) * 32 + l32;
+            const long long at = t < g.N ? rows.target[t] - m0 : -1;
+            const int want = at >= 0 && at < min(BM, g.M - m0) ? (int)at : -1;
+            float s = 0.f;
+            const float ref = mx[n] == -INFINITY ? 0.f : mx[n];       // all -inf: exp(-inf) = 0 each
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s += exp_of(acc[i][n][r] - ref);
+                    if (want == (wm * MI + i) * 32 + 8 * (r >> 2) + 4 * lh + (r & 3)) picked[t] = acc[i][n][r];
+                }
+            sum[n] = s;
+            const float mo = __shfl_xor(mx[n], 32), so = __shfl_xor(sum[n], 32);
+            stats_join(mx[n], sum[n], mo, so);
+        }
+        __builtin_amdgcn_s_barrier();                                  // every wave is done with the last stage
+        asm volatile("" ::: "memory");
+        float2* ex = reinterpret_cast<float2*>(lds);                   // [WM][BN]
+        if (lh == 0) {
+#pragma unroll
+            for (int n = 0; n < NI; ++n) ex[wm * BN + (wn * NI + n) * 32 + l32] = make_float2(mx[n], sum[n]);
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < BN; c += 64 * WM * WN) {
+            if (n0 + c >= g.N) continue;
+            float2 a = ex[c];
+#pragma unroll
+            for (int k = 1; k < WM; ++k) stats_join(a.x, a.y, ex[k * BN + c].x, ex[k * BN + c].y);
+            stats[(long)(m0 / BM) * g.N + n0 + c] = a;
+        }
+    }
+};
+
+// the weight of a row's gradient: 0 for an ignored row, NaN where the target is outside the vocabulary
+__device__ __forceinline__ float row_weight(const CeRows& rows, long long target, float grad) {
+    if (target == rows.ignore) return 0.f;
+    return target < 0 || target >= rows.V ? NAN : grad;
+}
+__device__ __forceinline__ float dl_of(float l, float lse, bool hit, float weight, bool ignored) {
+    return ignored ? 0.f : (exp_of(l - lse) - (hit ? 1.f : 0.f)) * weight;
+}
+
+// dl[t][v - v0] of a piece of the vocabulary, zeros around it (rows up to row_end, columns up to pitch)
+template <typename T> struct CeDl {
+    const T* bias;          // of the piece
+    CeRows rows;
+    const float* lse;
+    const float* grad;
+    const float* scale;     // one factor in device memory, or null
+    int v0;                 // first class of the piece
+    T* dl;
+    long pitch;             // elements, a multiple of 8
+    int row_end;
+    template <int BM, int BN, int WM, int WN, int MI, int NI>
+    __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char*) const {
+        const float f = scale ? *scale : 1.f;
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int t = n0 + (wn * NI + n) * 32 + l32;
+            if (t >= row_end) continue;
+            const bool in = t < g.N;
+            const long long target = in ? rows.target[t] : rows.ignore;
+            const bool ignored = !in || target == rows.ignore;
+            const float weight = in ? row_weight(rows, target, grad[t]) * f : 0.f;
+            const float z = in ? lse[t] : 0.f;
+            const int hit = target >= v0 && target - v0 < g.M ? (int)(target - v0) : -1;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int m = m0 + (wm * MI + i) * 32 + 8 * q + 4 * lh;
+                    if (m >= pitch) continue;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float b = bias && m + e < g.M ? to_f32(bias[m + e]) : 0.f;
+                        v[e] = m + e < g.M ? dl_of(acc[i][n][4 * q + e] + b, z, hit == m + e, weight, ignored) : 0.f;
+                    }
+                    store4<T>(dl + (long)t * pitch + m, v, 4, true);
+                }
+        }
+    }
+};
+
+// ---- kernels -----------------------------------------------------------------------------------
+
+// loss and lse from the tiles' statistics: 32 rows x 8 parts of the tile list per workgroup
+__global__ __launch_bounds__(256) static void ce_join_kernel(const float2* __restrict__ stats, const float* __restrict__ picked, CeRows rows,
+                                                             int T, int tiles, float* __restrict__ loss, float* __restrict__ lse) {
+    __shared__ float2 ex[8][32];
+    const int c = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int t = blockIdx.x * 32 + c;
+    float mx = -INFINITY, sum = 0.f;
+    if (t < T) {
+        for (int k = part; k < tiles; k += 8) {
+            const float2 a = stats[(long)k * T + t];
+            stats_join(mx, sum, a.x, a.y);
+        }
+    }
+    ex[part][c] = make_float2(mx, sum);
+    __syncthreads();
+    if (part != 0 || t >= T) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) stats_join(mx, sum, ex[k][c].x, ex[k][c].y);
+    const float z = mx + logf(sum);
+    const long long target = rows.target[t];
+    lse[t] = z;
+    loss[t] = target == rows.ignore ? 0.f : target < 0 || target >= rows.V ? NAN : z - picked[t];
+}
+
+// the logit from the partial sums of a cut reduction
+template <typename T> struct CeParts {
+    const float* part;
+    int parts;
+    long pitch, plane;      // elements per row, per part
+    const T* bias;
+    __device__ __forceinline__ float logit(long t, int v) const {
+        const float* at = part + t * pitch + v;
+        float s = 0.f;
+        for (int z = 0; z < parts; ++z) s += at[z * plane];
+        return s + (bias ? to_f32(bias[v]) : 0.f);
+    }
+};
+
+// small problems: loss and lse of one row per workgroup from the partial sums
+template <typename T>
+__global__ __launch_bounds__(256) void ce_rows_kernel(CeParts<T> p, CeRows rows, float* __restrict__ loss, float* __restrict__ lse) {
+    __shared__ float2 ex[256];
+    const int t = blockIdx.x;
+    float mx = -INFINITY, sum = 0.f;
+    for (int v = threadIdx.x; v < rows.V; v += 256) {
+        const float l = p.logit(t, v);
+        stats_join(mx, sum, l, l == -INFINITY ? 0.f : 1.f + (l - l));      // +inf and NaN make the row NaN
+    }
+    ex[threadIdx.x] = make_float2(mx, sum);
+    __syncthreads();
+    for (int k = 128; k > 0; k >>= 1) {
+        if ((int)threadIdx.x < k) {
+            stats_join(mx, sum, ex[threadIdx.x + k].x, ex[threadIdx.x + k].y);
+            ex[threadIdx.x] = make_float2(mx, sum);
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x != 0) return;
+    const float z = mx + logf(sum);
+    const long long target = rows.target[t];
+    lse[t] = z;
+    loss[t] = target == rows.ignore ? 0.f : target < 0 || target >= rows.V ? NAN : z - p.logit(t, (int)target);
+}
+
+// small problems: dl from the partial sums, four classes per thread
+template <typename T>
+__global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int T_rows) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const int quads = (int)(o.pitch / 4);
+    const int t = (int)(i / quads), m = (int)(i - (long)t * quads) * 4;
+    if (t >= o.row_end) return;
+    const bool in = t < T_rows;
+    const long long target = in ? o.rows.target[t] : o.rows.ignore;
+    const bool ignored = !in || target == o.rows.ignore;
+    const float weight = in ? row_weight(o.rows, target, o.grad[t]) * (o.scale ? *o.scale : 1.f) : 0.f;
+    const float z = in ? o.lse[t] : 0.f;
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = in && m + e < o.rows.V ? dl_of(p.logit(t, m + e), z, target == m + e, weight, ignored) : 0.f;
+    store4<T>(o.dl + (long)t * o.pitch + m, v, 4, true);
+}
+
+// dbias[v] = scale * sum_t dl[t][v], fp32, rows in a fixed order: 64 classes x 16 groups of rows per workgroup
+template <typename T>
+__global__ __launch_bounds__(1024) void ce_bias_kernel(const T* __restrict__ dl, long pitch, int rows, int V, const float* __restrict__ scale,
+                                                       T* __restrict__ dbias) {
+    __shared__ float ex[16][64];
+    const int c = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int v = blockIdx.x * 64 + c;
+    float s = 0.f;
+    if (v < V)
+        for (int t = part; t < rows; t += 16) s += to_f32(dl[(long)t * pitch + v]);
+    ex[part][c] = s;
+    __syncthreads();
+    if (part != 0 || v >= V) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += ex[k][c];
+    dbias[v] = from_f32<T>(s * (scale ? *scale : 1.f));
+}
+
+// f16 has five exponent bits: dl is stored times 2^(15 - e) with 2^e just above the largest weight, and the products
+// are multiplied back.  |exp(l - lse) - hit| <= 1, so nothing overflows (2^15 < 65504), and values down to 2^-39 of
+// the largest weight are kept.  out[0] = the factor, out[1] = its inverse; powers of two, so both are exact.
+__global__ __launch_bounds__(1024) static void ce_scale_kernel(const float* __restrict__ grad, CeRows rows, int T, float* __restrict__ out) {
+    __shared__ float ex[1024];
+    float mx = 0.f;
+    for (int t = threadIdx.x; t < T; t += 1024)
+        if (rows.target[t] != rows.ignore) mx = fmaxf(mx, fabsf(grad[t]));
+    ex[threadIdx.x] = mx;
+    __syncthreads();
+    for (int k = 512; k > 0; k >>= 1) {
+        if ((int)threadIdx.x < k) ex[threadIdx.x] = fmaxf(ex[threadIdx.x], ex[threadIdx.x + k]);
+        __syncthreads();
+    }
+    if (threadIdx.x != 0) return;
+    int e = 15;                                                        // no weight at all, or none that is finite: 1
+    if (ex[0] > 0.f && ex[0] <= 3.4028235e38f) {
+        frexpf(ex[0], &e);
+        e = max(e, -100);
+    }
+    out[0] = ldexpf(1.f, 15 - e);
+    out[1] = ldexpf(1.f, e - 15);
+}
+
+// rows of `cols` elements copied to a 16-byte aligned pitch, zeros behind them
+template <typename T>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ x, long rows, int cols, T* __restrict__ y, int pitch) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const int quads = pitch / 4;
+    const long row = i / quads;
+    if (row >= rows) return;
+    const int c = (int)(i - row * quads) * 4;
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? to_f32(x[row * cols + c + e]) : 0.f;
+    store4<T>(y + row * pitch + c, v, 4, true);
+}
+
+}  // namespace wino

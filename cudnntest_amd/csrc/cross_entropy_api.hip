@@ -1,0 +1,292 @@
+// C entry points of the softmax cross entropy (include/wino_amd.h).
+#include "cross_entropy.hpp"
+#include "host.hpp"
+
+using namespace wino;
+
+namespace {
+
+bool valid_dtype(int d) { return d == WINO_F32 || d == WINO_F16 || d == WINO_BF16; }
+bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+
+constexpr int kMaxCols = 1 << 21;                     // the kernels' 32-bit offsets inside a tile rest on it
+constexpr long kMaxTiles = 1L << 30;
+constexpr size_t kPieceBytes = 128u << 20;            // dl of one piece of the vocabulary: half of the last-level cache
+
+// Where everything is in the workspace, and how the problem is cut.  The same function sizes the workspace and drives
+// the calls.
+struct Plan {
+    bool pad_x, pad_w;                  // copied to 16-byte aligned rows first (odd lengths or bases)
+    int pitch_x, pitch_w;               // elements
+    bool small;                         // fewer tiles than CUs: logits as partial sums of a cut reduction
+    int parts;                          // of the logits' reduction (small)
+    int rows;                           // of dl: T rounded up to a stage
+    int piece;                          // classes per piece (backward)
+    int dx_parts, dw_parts;
+    size_t x, w, logits, stats, picked, scale, dl, dx, dw, total;
+};
+
+size_t place(size_t& at, size_t bytes) {
+    const size_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+}
+
+Plan plan(int dtype, int T, int D, int V, const void* x, const void* w, bool backward) {
+    Plan p = {};
+    const size_t e = dtype_size(dtype);
+    const int stage = (int)(128 / e), cus = device_cus();
+    const bool odd = (size_t)D * e % 16 != 0;
+    p.pad_x = odd || misaligned(x, 16);
+    p.pad_w = odd || misaligned(w, 16);
+    const int padded = (int)round_up(D, 8);
+    p.pitch_x = p.pad_x ? padded : D;
+    p.pitch_w = p.pad_w ? padded : D;
+    const int stages = ceil_div(D, stage);
+    p.small = (long)ceil_div(V, kTile) * ceil_div(T, kTile) < cus;
+    p.parts = p.small ? tile_parts(V, T, stages, cus) : 1;
+    size_t at = 0;
+    if (p.pad_x) p.x = place(at, (size_t)T * p.pitch_x * e);
+    if (p.pad_w) p.w = place(at, (size_t)V * p.pitch_w * e);
+    if (p.small) p.logits = place(at, part_bytes(V, T, p.parts));
+    if (!backward) {
+        if (!p.small) {
+            p.stats = place(at, (size_t)ceil_div(V, kTile) * T * sizeof(float2));
+            p.picked = place(at, (size_t)T * sizeof(float));
+        }
+    } else {
+        p.scale = place(at, 2 * sizeof(float));
+        p.rows = (int)round_up(T, 64);
+        const size_t fit = kPieceBytes / ((size_t)p.rows * e) / 256 * 256;
+        p.piece = p.small ? V : (int)std::min<size_t>(V, std::max<size_t>(fit, 256));
+        p.dl = place(at, (size_t)p.rows * round_up(p.piece, 128) * e);
+        p.dx_parts = tile_parts(D, T, ceil_div(p.piece, stage), cus);
+        p.dw_parts = tile_parts(D, p.piece, ceil_div(T, stage), cus);
+        if (p.dx_parts > 1 || p.piece < V) p.dx = place(at, part_bytes(D, T, p.dx_parts));
+        if (p.dw_parts > 1) p.dw = place(at, part_bytes(D, p.piece, p.dw_parts));
+    }
+    p.total = at;
+    return p;
+}
+
+int check(const char* what, int dtype, int T, int D, int V, const void* x, const void* w, const void* bias, const void* target) {
+    if (!valid_dtype(dtype)) return fail(WINO_ERR_INVALID, "%s: bad dtype %d", what, dtype);
+    if (T <= 0 || D <= 0 || V <= 0) return fail(WINO_ERR_INVALID, "%s: sizes must be positive (T %d, D %d, V %d)", what, T, D, V);
+    if (D > kMaxCols) return fail(WINO_ERR_UNSUPPORTED, "%s: D = %d, at most %d", what, D, kMaxCols);
+    if (V > (1 << 24)) return fail(WINO_ERR_UNSUPPORTED, "%s: V = %d, at most %d", what, V, 1 << 24);
+    if ((long)ceil_div(T, kTile) * ceil_div(V, kTile) > kMaxTiles || (long)ceil_div(T, kTile) * ceil_div(D, kTile) > kMaxTiles)
+        return fail(WINO_ERR_UNSUPPORTED, "%s: T = %d is too large", what, T);
+    if (!x || !w || !target) return fail(WINO_ERR_INVALID, "%s: null x, w or target", what);
+    const size_t e = dtype_size(dtype);
+    if (misaligned(x, e) || misaligned(w, e) || (bias && misaligned(bias, e)) || misaligned(target, 8))
+        return fail(WINO_ERR_INVALID, "%s: tensors must be aligned to their element type", what);
+    return WINO_OK;
+}
+
+template <typename T> TileOperand inner(const T* p, long pitch, int rows) {
+    const long b = pitch * (long)sizeof(T);
+    return {reinterpret_cast<const char*>(p), nullptr, b, 128, rows, 0};
+}
+template <typename T> TileOperand outer(const T* p, long pitch, int k_rows) {
+    const long b = pitch * (long)sizeof(T);
+    return {reinterpret_cast<const char*>(p), nullptr, b, b * TileElem<T>::stage, k_rows, (int)(b / 16)};
+}
+
+template <typename T> int pad_rows(const T* x, long rows, int cols, T* y, int pitch, hipStream_t s) {
+    const long n = rows * (pitch / 4);
+    if (ceil_div(n, 256) <= 0 || n / 256 > 0x7ffffff0L) return fail(WINO_ERR_UNSUPPORTED, "pad_rows: %ld rows of %d", rows, cols);
+    hipLaunchKernelGGL((pad_rows_kernel<T>), dim3(ceil_div(n, 256)), dim3(256), 0, s, x, rows, cols, y, pitch);
+    LAUNCH_CHECK("pad_rows");
+    return WINO_OK;
+}
+
+template <typename T> struct Call {
+    int T_, D, V;
+    const T *x, *w, *bias;
+    CeRows rows;
+    Plan p;
+    char* ws;
+    hipStream_t s;
+
+    int operands() {
+        if (p.pad_x) {
+            T* y = reinterpret_cast<T*>(ws + p.x);
+            const int rc = pad_rows<T>(x, T_, D, y, p.pitch_x, s);
+            if (rc) return rc;
+            x = y;
+        }
+        if (p.pad_w) {
+            T* y = reinterpret_cast<T*>(ws + p.w);
+            const int rc = pad_rows<T>(w, V, D, y, p.pitch_w, s);
+            if (rc) return rc;
+            w = y;
+        }
+        return WINO_OK;
+    }
+    TileArgs logits(int v0, int n) const {
+        TileArgs g = {};
+        g.a = inner<T>(w + (long)v0 * p.pitch_w, p.pitch_w, n);
+        g.b = inner<T>(x, p.pitch_x, T_);
+        g.M = n;
+        g.N = T_;
+        g.K = D;
+        return g;
+    }
+    int partial_logits(CeParts<T>* parts) {
+        float* to = reinterpret_cast<float*>(ws + p.logits);
+        const long pitch = round_up(V, 4);
+        tile_launch<T, K_INNER, K_INNER>(logits(0, V), TilePart{to, pitch, 0}, p.parts, s);
+        LAUNCH_CHECK("logits in parts");
+        *parts = {to, p.parts, pitch, pitch * T_, bias};
+        return WINO_OK;
+    }
+
+    int forward(float* loss, float* lse) {
+        int rc = operands();
+        if (rc) return rc;
+        if (p.small) {
+            CeParts<T> parts;
+            if ((rc = partial_logits(&parts))) return rc;
+            hipLaunchKernelGGL((ce_rows_kernel<T>), dim3(T_), dim3(256), 0, s, parts, rows, loss, lse);
+            LAUNCH_CHECK("ce_rows");
+            return WINO_OK;
+        }
+        float2* stats = reinterpret_cast<float2*>(ws + p.stats);
+        float* picked = reinterpret_cast<float*>(ws + p.picked);
+        tile_launch<T, K_INNER, K_INNER>(logits(0, V), CeStats<T>{bias, rows, stats, picked}, 1, s);
+        LAUNCH_CHECK("ce_stats");
+        hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(T_, 32)), dim3(256), 0, s, stats, picked, rows, T_, ceil_div(V, kTile), loss, lse);
+        LAUNCH_CHECK("ce_join");
+        return WINO_OK;
+    }
+
+    int backward(const float* grad, const float* lse, T* dx, T* dw, T* dbias) {
+        int rc = operands();
+        if (rc) return rc;
+        float* scale = nullptr;
+        if (std::is_same<T, f16_t>::value) {
+            scale = reinterpret_cast<float*>(ws + p.scale);
+            hipLaunchKernelGGL(ce_scale_kernel, dim3(1), dim3(1024), 0, s, grad, rows, T_, scale);
+            LAUNCH_CHECK("ce_scale");
+        }
+        const float* back = scale ? scale + 1 : nullptr;
+        T* dl = reinterpret_cast<T*>(ws + p.dl);
+        float* dx_part = reinterpret_cast<float*>(ws + p.dx);
+        float* dw_part = reinterpret_cast<float*>(ws + p.dw);
+        const bool dx_direct = p.dx_parts == 1 && p.piece >= V;
+        const long d4 = round_up(D, 4);
+        const TileStore<T> dx_store = {dx, D, nullptr, back, 0};
+        for (int v0 = 0; v0 < V; v0 += p.piece) {
+            const int n = std::min(p.piece, V - v0);
+            const long pitch = round_up(n, 128);
+            const CeDl<T> out = {bias ? bias + v0 : nullptr, rows, lse, grad, scale, v0, dl, pitch, p.rows};
+            if (p.small) {
+                CeParts<T> parts;
+                if ((rc = partial_logits(&parts))) return rc;
+                hipLaunchKernelGGL((ce_dl_kernel<T>), dim3(ceil_div((long)p.rows * (pitch / 4), 256)), dim3(256), 0, s, parts, out, T_);
+            } else {
+                tile_launch<T, K_INNER, K_INNER>(logits(v0, n), out, 1, s);
+            }
+            LAUNCH_CHECK("ce_dl");
+            if (dx) {                   // dx[t][d] (+)= sum_v w[v][d] dl[t][v]
+                TileArgs g = {};
+                g.a = outer<T>(w + (long)v0 * p.pitch_w, p.pitch_w, n);
+                g.b = inner<T>(dl, pitch, T_);
+                g.M = D;
+                g.N = T_;
+                g.K = n;
+                if (dx_direct) tile_launch<T, K_OUTER, K_INNER>(g, dx_store, 1, s);
+                else tile_launch<T, K_OUTER, K_INNER>(g, TilePart{dx_part, d4, v0 > 0}, p.dx_parts, s);
+                LAUNCH_CHECK("ce_dx");
+            }
+            if (dw) {                   // dw[v][d] = sum_t x[t][d] dl[t][v]
+                TileArgs g = {};
+                g.a = outer<T>(x, p.pitch_x, T_);
+                g.b = outer<T>(dl, pitch, p.rows);
+                g.M = D;
+                g.N = n;
+                g.K = T_;
+                const TileStore<T> store = {dw + (long)v0 * D, D, nullptr, back, 0};
+                if (p.dw_parts == 1) {
+                    tile_launch<T, K_OUTER, K_OUTER>(g, store, 1, s);
+                } else {
+                    tile_launch<T, K_OUTER, K_OUTER>(g, TilePart{dw_part, d4, 0}, p.dw_parts, s);
+                    LAUNCH_CHECK("ce_dw");
+                    hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(D, 4) * n, 256)), dim3(256), 0, s,
+                                       dw_part, p.dw_parts, d4, D, n, store);
+                }
+                LAUNCH_CHECK("ce_dw");
+            }
+            if (dbias) {
+                hipLaunchKernelGGL((ce_bias_kernel<T>), dim3(ceil_div(n, 64)), dim3(1024), 0, s, dl, pitch, T_, n, back, dbias + v0);
+                LAUNCH_CHECK("ce_bias");
+            }
+        }
+        if (dx && !dx_direct) {
+            hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(D, 4) * T_, 256)), dim3(256), 0, s, dx_part, p.dx_parts, d4, D, T_, dx_store);
+            LAUNCH_CHECK("ce_dx join");
+        }
+        return WINO_OK;
+    }
+};
+
+template <typename T>
+Call<T> make_call(int T_, int D, int V, const void* x, const void* w, const void* bias, const long long* target, long long ignore,
+                  const Plan& p, void* ws, void* stream) {
+    return {T_, D, V, static_cast<const T*>(x), static_cast<const T*>(w), static_cast<const T*>(bias), {target, ignore, V}, p,
+            static_cast<char*>(ws), (hipStream_t)stream};
+}
+
+int check_workspace(const char* what, const Plan& p, const void* ws, size_t bytes) {
+    if (p.total == 0) return WINO_OK;
+    if (!ws || bytes < p.total) return fail(WINO_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, ws ? bytes : 0, p.total);
+    if (misaligned(ws, 256)) return fail(WINO_ERR_INVALID, "%s: the workspace must be 256-byte aligned", what);
+    return WINO_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t wino_linear_cross_entropy_workspace_bytes(int dtype, int T, int D, int V, const void* x, const void* w, int backward) {
+    static const long long any = 0;
+    if (check("wino_linear_cross_entropy_workspace_bytes", dtype, T, D, V, x, w, nullptr, &any)) return 0;
+    return plan(dtype, T, D, V, x, w, backward != 0).total;
+}
+
+int wino_linear_cross_entropy(int dtype, int T, int D, int V, const void* x, const void* w, const void* bias, const long long* target,
+                              long long ignore_index, float* loss, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check("wino_linear_cross_entropy", dtype, T, D, V, x, w, bias, target);
+    if (rc) return rc;
+    if (!loss || !lse) return fail(WINO_ERR_INVALID, "wino_linear_cross_entropy: null loss or lse");
+    if (misaligned(loss, 4) || misaligned(lse, 4)) return fail(WINO_ERR_INVALID, "wino_linear_cross_entropy: loss and lse must be 4-byte aligned");
+    const Plan p = plan(dtype, T, D, V, x, w, false);
+    if ((rc = check_workspace("wino_linear_cross_entropy", p, workspace, workspace_bytes))) return rc;
+    if (dtype == WINO_F32) return make_call<float>(T, D, V, x, w, bias, target, ignore_index, p, workspace, stream).forward(loss, lse);
+    if (dtype == WINO_F16) return make_call<f16_t>(T, D, V, x, w, bias, target, ignore_index, p, workspace, stream).forward(loss, lse);
+    return make_call<bf16_t>(T, D, V, x, w, bias, target, ignore_index, p, workspace, stream).forward(loss, lse);
+}
+
+int wino_linear_cross_entropy_backward(int dtype, int T, int D, int V, const void* x, const void* w, const void* bias,
+                                       const long long* target, long long ignore_index, const float* grad, const float* lse, void* dx,
+                                       void* dw, void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check("wino_linear_cross_entropy_backward", dtype, T, D, V, x, w, bias, target);
+    if (rc) return rc;
+    if (!grad || !lse) return fail(WINO_ERR_INVALID, "wino_linear_cross_entropy_backward: null grad or lse");
+    if (!dx && !dw && !dbias) return fail(WINO_ERR_INVALID, "wino_linear_cross_entropy_backward: no gradient asked for");
+    const size_t e = dtype_size(dtype);
+    if (misaligned(grad, 4) || misaligned(lse, 4) || misaligned(dx, e) || misaligned(dw, e) || misaligned(dbias, e))
+        return fail(WINO_ERR_INVALID, "wino_linear_cross_entropy_backward: tensors must be aligned to their element type");
+    const Plan p = plan(dtype, T, D, V, x, w, true);
+    if ((rc = check_workspace("wino_linear_cross_entropy_backward", p, workspace, workspace_bytes))) return rc;
+    if (dtype == WINO_F32)
+        return make_call<float>(T, D, V, x, w, bias, target, ignore_index, p, workspace, stream)
+            .backward(grad, lse, static_cast<float*>(dx), static_cast<float*>(dw), static_cast<float*>(dbias));
+    if (dtype == WINO_F16)
+        return make_call<f16_t>(T, D, V, x, w, bias, target, ignore_index, p, workspace, stream)
+            .backward(grad, lse, static_cast<f16_t*>(dx), static_cast<f16_t*>(dw), static_cast<f16_t*>(dbias));
+    return make_call<bf16_t>(T, D, V, x, w, bias, target, ignore_index, p, workspace, stream)
+        .backward(grad, lse, static_cast<bf16_t*>(dx), static_cast<bf16_t*>(dw), static_cast<bf16_t*>(dbias));
+}
+
+}  // extern "C"

@@ -17,6 +17,7 @@
 #include "direct16_rows.hpp"
 #include "gemm.hpp"
 #include "gemm_rows_f4.hpp"
+#include "host.hpp"
 #include "transforms.hpp"
 #include "transforms_f4.hpp"
 
@@ -26,8 +27,8 @@ using namespace wino;
 // process ends.  In host code this name is only a handle for hipGetSymbolAddress (see noalloc_scratch below).
 static __device__ __align__(256) unsigned char scratch[WINO_NOALLOC_SCRATCH_BYTES];
 
-namespace {
-
+// the calling thread's last failure (host.hpp)
+namespace wino {
 thread_local char g_err[512] = "";
 
 int fail(int code, const char* fmt, ...) {
@@ -37,27 +38,6 @@ int fail(int code, const char* fmt, ...) {
     va_end(ap);
     return code;
 }
-
-#define HIP_TRY(expr)                                                                            \
-    do {                                                                                         \
-        hipError_t e_ = (expr);                                                                  \
-        if (e_ != hipSuccess) return fail(WINO_ERR_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
-    } while (0)
-
-#define LAUNCH_CHECK(name)                                                                        \
-    do {                                                                                          \
-        hipError_t e_ = hipGetLastError();                                                        \
-        if (e_ != hipSuccess) return fail(WINO_ERR_HIP, "launch %s: %s", name, hipGetErrorString(e_)); \
-    } while (0)
-
-bool valid_layout(int l) { return l == WINO_NCHW || l == WINO_NHWC || l == WINO_CHWN; }
-bool valid_dtype(int d) { return d == WINO_F32 || d == WINO_F16 || d == WINO_BF16; }
-bool valid_porder(int o) { return o == WINO_PRODUCT_KP || o == WINO_PRODUCT_PK; }
-// Winograd-domain operands (U, V, M) move as 16-byte vectors, partly by direct-to-LDS loads: their addresses
-// must be 16-byte aligned (every hipMalloc'ed buffer is); plain tensors need their element's alignment only.
-bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
-size_t elem_bytes(int dtype) { return dtype == WINO_F32 ? 4 : 2; }
-bool valid_order(int o) { return o == WINO_TILES_BATCH_MAJOR || o == WINO_TILES_BATCH_MINOR; }
 
 constexpr int kMaxDevices = 16;
 
@@ -75,6 +55,19 @@ int device_cus() {
     }
     return cus[dev];
 }
+}  // namespace wino
+
+namespace {
+
+bool valid_layout(int l) { return l == WINO_NCHW || l == WINO_NHWC || l == WINO_CHWN; }
+bool valid_dtype(int d) { return d == WINO_F32 || d == WINO_F16 || d == WINO_BF16; }
+bool valid_porder(int o) { return o == WINO_PRODUCT_KP || o == WINO_PRODUCT_PK; }
+// Winograd-domain operands (U, V, M) move as 16-byte vectors, partly by direct-to-LDS loads: their addresses
+// must be 16-byte aligned (every hipMalloc'ed buffer is); plain tensors need their element's alignment only.
+bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+size_t elem_bytes(int dtype) { return dtype == WINO_F32 ? 4 : 2; }
+bool valid_order(int o) { return o == WINO_TILES_BATCH_MAJOR || o == WINO_TILES_BATCH_MINOR; }
+
 // workgroups of the row-at-a-time GEMM resident at once: 2 per CU (64 KB of LDS, fp32) or 3 (48 KB, 2-byte operands)
 long rows_slots(int dtype) { return (long)device_cus() * (dtype == WINO_F32 ? 2 : 3); }
 

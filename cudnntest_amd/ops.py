@@ -389,6 +389,191 @@ def layout_transform(t, src, dst):
     return out
 
 
+# ---- the network's head: 4-bit fully connected layers, softmax cross entropy ------------------
+
+def _on(device, *tensors):
+    """Contiguous tensors of one GPU; None passes.  Their addresses."""
+    out = []
+    for t in tensors:
+        if t is None:
+            out.append(None)
+            continue
+        if t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
+        out.append(_ptr(t))
+    return out
+
+
+def _matrix(t, what):
+    if t.dim() != 2:
+        raise ValueError(f"{what} must be a matrix, got {t.dim()} dimensions")
+    return t.shape
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _out_as(out, shape, dtype, device):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise ValueError(f"out is {tuple(out.shape)} of {out.dtype}, the call writes {tuple(shape)} of {dtype}")
+    return out
+
+
+def _check_row_bias(bias, n, dtype):
+    if bias is not None and (bias.dtype != dtype or bias.numel() != n):
+        raise TypeError(f"bias must hold {n} elements of {dtype}")
+
+
+class Mx4:
+    """A matrix [rows][K] in microscaled 4-bit floating point (what wino_mx4_quantize writes): `codes`
+    uint8 [Kp/256][rows][128], two elements a byte, and `scales` uint8 [Kp/256][rows rounded up to 2][8],
+    one power-of-two exponent per 32 columns; Kp is K rounded up to 256."""
+
+    def __init__(self, codes, scales, rows, K):
+        want = mx4_geometry(rows, K)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales are uint8")
+        if codes.numel() != want["code_bytes"] or scales.numel() != want["scale_bytes"]:
+            raise ValueError(f"a {rows} x {K} matrix has {want['code_bytes']} bytes of codes and {want['scale_bytes']} of "
+                             f"scales, got {codes.numel()} and {scales.numel()}")
+        self.codes, self.scales, self.rows, self.K = codes, scales, int(rows), int(K)
+
+    @property
+    def shape(self):
+        return (self.rows, self.K)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def mx4_geometry(rows, K):
+    import ctypes
+    kp, cb, sb = ctypes.c_int(), ctypes.c_size_t(), ctypes.c_size_t()
+    _lib.check(_lib.load().wino_mx4_geometry(rows, K, kp, cb, sb), "wino_mx4_geometry")
+    return dict(Kp=kp.value, code_bytes=cb.value, scale_bytes=sb.value)
+
+
+def mx4_quantize(x, out=None):
+    """x [rows][K] in microscaled 4 bits; `out` an Mx4 of the same shape to write into.  Asynchronous."""
+    rows, K = _matrix(x, "x")
+    dt = _dt(x)
+    px, = _on(x.device, x)
+    if out is None:
+        g = mx4_geometry(rows, K)
+        out = Mx4(torch.empty((g["Kp"] // 256, rows, 128), dtype=torch.uint8, device=x.device),
+                  torch.empty((g["Kp"] // 256, (rows + 1) // 2 * 2, 8), dtype=torch.uint8, device=x.device), rows, K)
+    elif out.shape != (rows, K):
+        raise ValueError(f"out holds {out.shape}, x is {(rows, K)}")
+    pc, ps = _on(x.device, out.codes, out.scales)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().wino_mx4_quantize(dt, rows, K, px, pc, ps, _stream()), "wino_mx4_quantize")
+    return out
+
+
+def mx4_dequantize(q, dtype=torch.float32, out=None):
+    """The values that q's codes stand for, [rows][K] of `dtype`."""
+    if dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {dtype}")
+    pc, ps = _on(q.device, q.codes, q.scales)
+    out = _out_as(out, q.shape, dtype, q.device)
+    po, = _on(q.device, out)
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.load().wino_mx4_dequantize(_DTYPES[dtype], q.rows, q.K, pc, ps, po, _stream()), "wino_mx4_dequantize")
+    return out
+
+
+def mx4_gemm(x, w, bias=None, relu=False, dtype=torch.float32, out=None):
+    """y = relu?(x w^T + bias) of two Mx4 matrices [M][K] and [N][K]; y and bias of `dtype`.  Asynchronous."""
+    if dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {dtype}")
+    if x.K != w.K:
+        raise ValueError(f"x has {x.K} columns, w has {w.K}")
+    M, N, K = x.rows, w.rows, w.K
+    _check_row_bias(bias, N, dtype)
+    out = _out_as(out, (M, N), dtype, x.device)
+    xc, xs, wc, ws, pb, po = _on(x.device, x.codes, x.scales, w.codes, w.scales, bias, out)
+    with torch.cuda.device(x.device):
+        L = _lib.load()
+        work = _workspace(L.wino_mx4_workspace_bytes(M, N, K), x.device)
+        _lib.check(L.wino_mx4_gemm(_DTYPES[dtype], FLAG_RELU if relu else 0, M, N, K, xc, xs, wc, ws, pb, po,
+                                   work.data_ptr(), work.numel(), _stream()), "wino_mx4_gemm")
+    return out
+
+
+def mx4_linear(x, w, bias=None, relu=False, out=None):
+    """y = relu?(x w^T + bias): a fully connected layer with 4-bit weights w (Mx4 [N][K]) on x [M][K], which is
+    quantised on the way in: the bits of mx4_gemm(mx4_quantize(x), w, bias, relu, x.dtype).  Asynchronous."""
+    M, K = _matrix(x, "x")
+    if K != w.K:
+        raise ValueError(f"x has {K} columns, w has {w.K}")
+    N, dt = w.rows, _dt(x)
+    _check_row_bias(bias, N, x.dtype)
+    out = _out_as(out, (M, N), x.dtype, x.device)
+    px, wc, ws, pb, po = _on(x.device, x, w.codes, w.scales, bias, out)
+    with torch.cuda.device(x.device):
+        L = _lib.load()
+        work = _workspace(L.wino_mx4_workspace_bytes(M, N, K), x.device)
+        _lib.check(L.wino_mx4_linear(dt, FLAG_RELU if relu else 0, M, N, K, px, wc, ws, pb, po, work.data_ptr(),
+                                     work.numel(), _stream()), "wino_mx4_linear")
+    return out
+
+
+def _ce_arguments(x, w, target, bias):
+    T, D = _matrix(x, "x")
+    V, D2 = _matrix(w, "w")
+    if D2 != D:
+        raise ValueError(f"x has {D} columns, w has {D2}")
+    if w.dtype != x.dtype:
+        raise TypeError("x and w must share a dtype")
+    if target.dtype != torch.int64 or tuple(target.shape) != (T,):
+        raise TypeError(f"target must be int64 of shape {(T,)}")
+    _check_row_bias(bias, V, x.dtype)
+    return T, D, V
+
+
+def linear_cross_entropy(x, w, target, bias=None, ignore_index=-100):
+    """Softmax cross entropy of the logits x w^T + bias against target, per row, without the logits in memory.
+    x [T][D], w [V][D], bias [V], target int64 [T] -> (loss [T], lse [T]) fp32; rows whose target is ignore_index
+    have loss 0, a target outside the classes gives NaN.  lse goes into linear_cross_entropy_backward.  Asynchronous."""
+    T, D, V = _ce_arguments(x, w, target, bias)
+    dt, dev = _dt(x), x.device
+    px, pw, pb, pt = _on(dev, x, w, bias, target)
+    loss, lse = torch.empty(2, T, dtype=torch.float32, device=dev).unbind(0)
+    with torch.cuda.device(dev):
+        L = _lib.load()
+        work = _workspace(L.wino_linear_cross_entropy_workspace_bytes(dt, T, D, V, px, pw, 0), dev)
+        _lib.check(L.wino_linear_cross_entropy(dt, T, D, V, px, pw, pb, pt, ignore_index, loss.data_ptr(), lse.data_ptr(),
+                                               work.data_ptr() if work is not None else None,
+                                               work.numel() if work is not None else 0, _stream()), "wino_linear_cross_entropy")
+    return loss, lse
+
+
+def linear_cross_entropy_backward(grad, x, w, target, lse, bias=None, ignore_index=-100, need=(True, True, True)):
+    """Gradients of sum_t grad[t] * loss[t] with respect to x, w and bias (None without a bias): grad and lse fp32 [T],
+    lse from linear_cross_entropy.  need: which of the three to compute, None in the others' place.  Asynchronous."""
+    T, D, V = _ce_arguments(x, w, target, bias)
+    dt, dev = _dt(x), x.device
+    for t, name in ((grad, "grad"), (lse, "lse")):
+        if t.dtype != torch.float32 or tuple(t.shape) != (T,):
+            raise TypeError(f"{name} must be float32 of shape {(T,)}")
+    px, pw, pb, pt, pg, pl = _on(dev, x, w, bias, target, grad, lse)
+    dx = torch.empty_like(x) if need[0] else None
+    dw = torch.empty_like(w) if need[1] else None
+    db = torch.empty(V, dtype=x.dtype, device=dev) if need[2] and bias is not None else None
+    if dx is None and dw is None and db is None:
+        return dx, dw, db
+    with torch.cuda.device(dev):
+        L = _lib.load()
+        work = _workspace(L.wino_linear_cross_entropy_workspace_bytes(dt, T, D, V, px, pw, 1), dev)
+        _lib.check(L.wino_linear_cross_entropy_backward(dt, T, D, V, px, pw, pb, pt, ignore_index, pg, pl, *_on(dev, dx, dw, db),
+                                                        work.data_ptr(), work.numel(), _stream()), "wino_linear_cross_entropy_backward")
+    return dx, dw, db
+
+
 # ---- the reference's call surface --------------------------------------------------------
 
 def _wrapped(src, dst, bat4Conv, inside, chn, numOfFilter, padding, m1, m2, output):

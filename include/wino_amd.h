@@ -286,8 +286,8 @@ int wino_stage_stats(float *sum_ms, float *min_ms, float *max_ms, long *calls);
  * poolForward after some layers -- here one wino_conv_prepared_ex call per layer, with bias, ReLU and
  * pooling in its output stage, the filter bank of every layer transformed once when it is set (the
  * reference transforms it again on every call), and the activations between layers in two buffers the
- * stack owns.  The fully connected layers and the softmax of the reference driver are cuBLAS/cuDNN
- * code and not part of this library.  Every layer is 3x3, stride 1, pad 1. */
+ * stack owns.  The fully connected layers and the softmax that follow are the head's calls further
+ * down.  Every layer is 3x3, stride 1, pad 1. */
 typedef struct wino_stack wino_stack_t;
 typedef struct {
     int K;                     /* filters of the layer; its channels are the previous layer's K */
@@ -313,6 +313,60 @@ int wino_stack_forward(wino_stack_t *stack, const void *x, void *y, void *stream
  * (VGG_Batched/Network.h:603-669) and has no counterpart. */
 int wino_stack_forward_graph(wino_stack_t *stack, const void *x, void *y, void *stream);
 int wino_stack_destroy(wino_stack_t *stack);
+
+/* ---- the network's head: 4-bit fully connected layers, and the softmax cross entropy ------------------------
+ * What follows the convolution stack in the reference's driver (fullyConnectedForward and softmaxForward,
+ * netTest/cudnn_test_0124/VGG_Batched/Network.h:145,603-669, cuBLAS / cuDNN there): fully connected layers with weights in
+ * microscaled 4-bit floating point, and the loss of the last layer with its gradient.  No counterpart in the reference.
+ *
+ * These calls use only the buffers they are given: calls on different streams may overlap if their workspaces and outputs
+ * are different buffers.  They allocate nothing, never synchronise, record no memset and can be captured into a graph.
+ * Results do not depend on timing: sums that are cut are joined in a fixed order.  The device that owns the buffers must
+ * be the current one.  Matrices are row-major and contiguous.
+ *
+ * Microscaled 4-bit format (OCP MX, e2m1 elements): along a row, 32 values share a scale 2^(b - 127), b one byte; elements
+ * are 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives.  A block with largest magnitude a gets b = clamp(floor(log2 a) + 125,
+ * 0, 254) and elements round(x / scale), to nearest with ties to even, saturating at 6.  A block that holds a NaN or an
+ * infinity gets b = 255 and stands for NaNs.  A matrix of `rows` x K, Kp = K rounded up to 256, is kept as
+ *     codes  [Kp/256][rows][128]                      two elements per byte, the lower column in the low four bits
+ *     scales [Kp/256][rows rounded up to 2][8]
+ * with zeros in the columns past K.  Both must be 16-byte aligned. */
+int wino_mx4_geometry(int rows, int K, int *Kp, size_t *code_bytes, size_t *scale_bytes);
+/* x [rows][K] of `dtype` (a wino_dtype_t) to 4 bits, and the values that the codes stand for back to `dtype` (exact in
+ * fp32 and bf16; in f16 values below its range are rounded, values above it become infinite) */
+int wino_mx4_quantize(int dtype, int rows, int K, const void *x, void *codes, void *scales, void *stream);
+int wino_mx4_dequantize(int dtype, int rows, int K, const void *codes, const void *scales, void *x, void *stream);
+/* bytes of workspace that wino_mx4_gemm and wino_mx4_linear need for these sizes (0 for invalid ones); 256-byte aligned */
+size_t wino_mx4_workspace_bytes(int M, int N, int K);
+/* y[m][n] = relu?( sum_k x[m][k] w[n][k] + bias[n] ): both matrices quantised; products of 4-bit values are exact, sums are
+ * fp32, y and bias (N elements or NULL) are of `dtype`.  flags: 0 or WINO_FLAG_RELU. */
+int wino_mx4_gemm(int dtype, unsigned flags, int M, int N, int K, const void *xcodes, const void *xscales, const void *wcodes,
+                  const void *wscales, const void *bias, void *y, void *workspace, size_t workspace_bytes, void *stream);
+/* The same with x [M][K] given in `dtype` and quantised on the way in: the bits of wino_mx4_quantize + wino_mx4_gemm. */
+int wino_mx4_linear(int dtype, unsigned flags, int M, int N, int K, const void *x, const void *wcodes, const void *wscales,
+                    const void *bias, void *y, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Softmax cross entropy of the logits l = x w^T + bias of a last layer (x [T][D], w [V][D], bias V elements or NULL, all of
+ * `dtype`), row by row, without the logits in memory:
+ *     lse[t] = log sum_v exp l[t][v],   loss[t] = lse[t] - l[t][target[t]]                              (both fp32)
+ * A row whose target is ignore_index has loss 0 (its lse is computed all the same); a target outside [0, V) that is not
+ * ignore_index makes the row's loss NaN.  Logits of -infinity (from the bias) mask their class; a row in which they all are
+ * has lse -infinity and loss NaN; a logit that is NaN or +infinity makes its row NaN.
+ * x and w are read in place when their rows are 16-byte aligned (D times the element size and both base addresses), and
+ * copied to aligned rows in the workspace otherwise: the workspace query takes the addresses of the call to come. */
+size_t wino_linear_cross_entropy_workspace_bytes(int dtype, int T, int D, int V, const void *x, const void *w, int backward);
+int wino_linear_cross_entropy(int dtype, int T, int D, int V, const void *x, const void *w, const void *bias,
+                              const long long *target, long long ignore_index, float *loss, float *lse, void *workspace,
+                              size_t workspace_bytes, void *stream);
+/* Gradients of sum_t grad[t] * loss[t], lse from the call above: with dl[t][v] = grad[t] (exp(l[t][v] - lse[t]) -
+ * [v == target[t]]) (zeros for an ignored row, NaN for a row with an invalid target)
+ *     dx = dl w,   dw = dl^T x,   dbias[v] = sum_t dl[t][v]
+ * in `dtype`; any of the three may be NULL.  The logits are computed again, a piece of the vocabulary at a time; dl is rounded
+ * to `dtype` before the products (in f16 scaled by a power of two taken from the largest weight, so that small probabilities
+ * do not underflow), sums are fp32. */
+int wino_linear_cross_entropy_backward(int dtype, int T, int D, int V, const void *x, const void *w, const void *bias,
+                                       const long long *target, long long ignore_index, const float *grad, const float *lse,
+                                       void *dx, void *dw, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- housekeeping ----------------------------------------------------------- */
 int wino_warmup(void);                 /* empty kernel; replaces warmup<<<1,1>>> (wrapedConv_NCHW.cuh:4-7) */
