@@ -157,7 +157,15 @@ __global__ __launch_bounds__(256) static void ce_join_kernel(const float2* __res
     const int t = blockIdx.x * 32 + c;
     float mx = -INFINITY, sum = 0.f;
     if (t < T) {
-        for (int k = part; k < tiles; k += 8) {
+        int k = part;
+        for (; k + 24 < tiles; k += 32) {                              // four loads in flight
+            float2 a[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) a[u] = stats[(long)(k + 8 * u) * T + t];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) stats_join(mx, sum, a[u].x, a[u].y);
+        }
+        for (; k < tiles; k += 8) {
             const float2 a = stats[(long)k * T + t];
             stats_join(mx, sum, a.x, a.y);
         }
@@ -181,9 +189,7 @@ template <typename T> struct CeParts {
     const T* bias;
     __device__ __forceinline__ float logit(long t, int v) const {
         const float* at = part + t * pitch + v;
-        float s = 0.f;
-        for (int z = 0; z < parts; ++z) s += at[z * plane];
-        return s + (bias ? to_f32(bias[v]) : 0.f);
+        return sum_parts<float>(at, parts, plane) + (bias ? to_f32(bias[v]) : 0.f);
     }
 };
 
@@ -239,8 +245,17 @@ __global__ __launch_bounds__(1024) void ce_bias_kernel(const T* __restrict__ dl,
     const int c = threadIdx.x & 63, part = threadIdx.x >> 6;
     const int v = blockIdx.x * 64 + c;
     float s = 0.f;
-    if (v < V)
-        for (int t = part; t < rows; t += 16) s += to_f32(dl[(long)t * pitch + v]);
+    if (v < V) {
+        int t = part;
+        for (; t + 112 < rows; t += 128) {                             // eight loads in flight
+            float a[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) a[u] = to_f32(dl[(long)(t + 16 * u) * pitch + v]);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += a[u];
+        }
+        for (; t < rows; t += 16) s += to_f32(dl[(long)t * pitch + v]);
+    }
     ex[part][c] = s;
     __syncthreads();
     if (part != 0 || v >= V) return;

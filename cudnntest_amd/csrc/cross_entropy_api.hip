@@ -18,11 +18,10 @@ constexpr size_t kPieceBytes = 128u << 20;            // dl of one piece of the 
 struct Plan {
     bool pad_x, pad_w;                  // copied to 16-byte aligned rows first (odd lengths or bases)
     int pitch_x, pitch_w;               // elements
-    bool small;                         // fewer tiles than CUs: logits as partial sums of a cut reduction
-    int parts;                          // of the logits' reduction (small)
+    bool small;                         // too few tiles for the chip: logits as partial sums of a cut reduction
+    TilePick logit, dx_cut, dw_cut;     // how the three products are cut
     int rows;                           // of dl: T rounded up to a stage
     int piece;                          // classes per piece (backward)
-    int dx_parts, dw_parts;
     size_t x, w, logits, stats, picked, scale, dl, dx, dw, total;
 };
 
@@ -32,26 +31,27 @@ size_t place(size_t& at, size_t bytes) {
     return here;
 }
 
-Plan plan(int dtype, int T, int D, int V, const void* x, const void* w, bool backward) {
+constexpr int kMostParts = 64;
+
+template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x, const void* w, bool backward) {
     Plan p = {};
     const size_t e = dtype_size(dtype);
-    const int stage = (int)(128 / e), cus = device_cus();
+    const int cus = device_cus();
     const bool odd = (size_t)D * e % 16 != 0;
     p.pad_x = odd || misaligned(x, 16);
     p.pad_w = odd || misaligned(w, 16);
     const int padded = (int)round_up(D, 8);
     p.pitch_x = p.pad_x ? padded : D;
     p.pitch_w = p.pad_w ? padded : D;
-    const int stages = ceil_div(D, stage);
-    p.small = (long)ceil_div(V, kTile) * ceil_div(T, kTile) < cus;
-    p.parts = p.small ? tile_parts(V, T, stages, cus) : 1;
+    p.logit = tile_pick<E>(V, T, D, kMostParts, cus);
+    p.small = p.logit.parts > 1;
     size_t at = 0;
     if (p.pad_x) p.x = place(at, (size_t)T * p.pitch_x * e);
     if (p.pad_w) p.w = place(at, (size_t)V * p.pitch_w * e);
-    if (p.small) p.logits = place(at, part_bytes(V, T, p.parts));
+    if (p.small) p.logits = place(at, part_bytes(V, T, p.logit.parts));
     if (!backward) {
         if (!p.small) {
-            p.stats = place(at, (size_t)ceil_div(V, kTile) * T * sizeof(float2));
+            p.stats = place(at, (size_t)ceil_div(V, p.logit.edge()) * T * sizeof(float2));
             p.picked = place(at, (size_t)T * sizeof(float));
         }
     } else {
@@ -60,13 +60,19 @@ Plan plan(int dtype, int T, int D, int V, const void* x, const void* w, bool bac
         const size_t fit = kPieceBytes / ((size_t)p.rows * e) / 256 * 256;
         p.piece = p.small ? V : (int)std::min<size_t>(V, std::max<size_t>(fit, 256));
         p.dl = place(at, (size_t)p.rows * round_up(p.piece, 128) * e);
-        p.dx_parts = tile_parts(D, T, ceil_div(p.piece, stage), cus);
-        p.dw_parts = tile_parts(D, p.piece, ceil_div(T, stage), cus);
-        if (p.dx_parts > 1 || p.piece < V) p.dx = place(at, part_bytes(D, T, p.dx_parts));
-        if (p.dw_parts > 1) p.dw = place(at, part_bytes(D, p.piece, p.dw_parts));
+        if (!p.small) p.logit = tile_pick<E>(p.piece, T, D, 1, cus);
+        p.dx_cut = tile_pick<E>(D, T, p.piece, kMostParts, cus);
+        p.dw_cut = tile_pick<E>(D, p.piece, T, kMostParts, cus);
+        if (p.dx_cut.parts > 1 || p.piece < V) p.dx = place(at, part_bytes(D, T, p.dx_cut.parts));
+        if (p.dw_cut.parts > 1) p.dw = place(at, part_bytes(D, p.piece, p.dw_cut.parts));
     }
     p.total = at;
     return p;
+}
+Plan plan(int dtype, int T, int D, int V, const void* x, const void* w, bool backward) {
+    return dtype == WINO_F32   ? plan_as<float>(dtype, T, D, V, x, w, backward)
+           : dtype == WINO_F16 ? plan_as<f16_t>(dtype, T, D, V, x, w, backward)
+                               : plan_as<bf16_t>(dtype, T, D, V, x, w, backward);
 }
 
 int check(const char* what, int dtype, int T, int D, int V, const void* x, const void* w, const void* bias, const void* target) {
@@ -135,9 +141,9 @@ template <typename T> struct Call {
     int partial_logits(CeParts<T>* parts) {
         float* to = reinterpret_cast<float*>(ws + p.logits);
         const long pitch = round_up(V, 4);
-        tile_launch<T, K_INNER, K_INNER>(logits(0, V), TilePart{to, pitch, 0}, p.parts, s);
+        tile_launch<T, K_INNER, K_INNER>(logits(0, V), TilePart{to, pitch, 0}, p.logit, T_, s);
         LAUNCH_CHECK("logits in parts");
-        *parts = {to, p.parts, pitch, pitch * T_, bias};
+        *parts = {to, p.logit.parts, pitch, pitch * T_, bias};
         return WINO_OK;
     }
 
@@ -153,9 +159,9 @@ template <typename T> struct Call {
         }
         float2* stats = reinterpret_cast<float2*>(ws + p.stats);
         float* picked = reinterpret_cast<float*>(ws + p.picked);
-        tile_launch<T, K_INNER, K_INNER>(logits(0, V), CeStats<T>{bias, rows, stats, picked}, 1, s);
+        tile_launch<T, K_INNER, K_INNER>(logits(0, V), CeStats<T>{bias, rows, stats, picked}, p.logit, T_, s);
         LAUNCH_CHECK("ce_stats");
-        hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(T_, 32)), dim3(256), 0, s, stats, picked, rows, T_, ceil_div(V, kTile), loss, lse);
+        hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(T_, 32)), dim3(256), 0, s, stats, picked, rows, T_, ceil_div(V, p.logit.edge()), loss, lse);
         LAUNCH_CHECK("ce_join");
         return WINO_OK;
     }
@@ -173,7 +179,7 @@ template <typename T> struct Call {
         T* dl = reinterpret_cast<T*>(ws + p.dl);
         float* dx_part = reinterpret_cast<float*>(ws + p.dx);
         float* dw_part = reinterpret_cast<float*>(ws + p.dw);
-        const bool dx_direct = p.dx_parts == 1 && p.piece >= V;
+        const bool dx_direct = p.dx_cut.parts == 1 && p.piece >= V;
         const long d4 = round_up(D, 4);
         const TileStore<T> dx_store = {dx, D, nullptr, back, 0};
         for (int v0 = 0; v0 < V; v0 += p.piece) {
@@ -185,7 +191,7 @@ template <typename T> struct Call {
                 if ((rc = partial_logits(&parts))) return rc;
                 hipLaunchKernelGGL((ce_dl_kernel<T>), dim3(ceil_div((long)p.rows * (pitch / 4), 256)), dim3(256), 0, s, parts, out, T_);
             } else {
-                tile_launch<T, K_INNER, K_INNER>(logits(v0, n), out, 1, s);
+                tile_launch<T, K_INNER, K_INNER>(logits(v0, n), out, p.logit, p.rows, s);
             }
             LAUNCH_CHECK("ce_dl");
             if (dx) {                   // dx[t][d] (+)= sum_v w[v][d] dl[t][v]
@@ -195,8 +201,8 @@ template <typename T> struct Call {
                 g.M = D;
                 g.N = T_;
                 g.K = n;
-                if (dx_direct) tile_launch<T, K_OUTER, K_INNER>(g, dx_store, 1, s);
-                else tile_launch<T, K_OUTER, K_INNER>(g, TilePart{dx_part, d4, v0 > 0}, p.dx_parts, s);
+                if (dx_direct) tile_launch<T, K_OUTER, K_INNER>(g, dx_store, p.dx_cut, T_, s);
+                else tile_launch<T, K_OUTER, K_INNER>(g, TilePart{dx_part, d4, v0 > 0}, p.dx_cut, T_, s);
                 LAUNCH_CHECK("ce_dx");
             }
             if (dw) {                   // dw[v][d] = sum_t x[t][d] dl[t][v]
@@ -207,13 +213,13 @@ template <typename T> struct Call {
                 g.N = n;
                 g.K = T_;
                 const TileStore<T> store = {dw + (long)v0 * D, D, nullptr, back, 0};
-                if (p.dw_parts == 1) {
-                    tile_launch<T, K_OUTER, K_OUTER>(g, store, 1, s);
+                if (p.dw_cut.parts == 1) {
+                    tile_launch<T, K_OUTER, K_OUTER>(g, store, p.dw_cut, n, s);
                 } else {
-                    tile_launch<T, K_OUTER, K_OUTER>(g, TilePart{dw_part, d4, 0}, p.dw_parts, s);
+                    tile_launch<T, K_OUTER, K_OUTER>(g, TilePart{dw_part, d4, 0}, p.dw_cut, n, s);
                     LAUNCH_CHECK("ce_dw");
                     hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(D, 4) * n, 256)), dim3(256), 0, s,
-                                       dw_part, p.dw_parts, d4, D, n, store);
+                                       dw_part, p.dw_cut.parts, d4, D, n, store);
                 }
                 LAUNCH_CHECK("ce_dw");
             }
@@ -223,7 +229,7 @@ template <typename T> struct Call {
             }
         }
         if (dx && !dx_direct) {
-            hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(D, 4) * T_, 256)), dim3(256), 0, s, dx_part, p.dx_parts, d4, D, T_, dx_store);
+            hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(D, 4) * T_, 256)), dim3(256), 0, s, dx_part, p.dx_cut.parts, d4, D, T_, dx_store);
             LAUNCH_CHECK("ce_dx join");
         }
         return WINO_OK;

@@ -50,8 +50,11 @@ TileOperand mx4_operand(const void* codes, const void* scales, int rows) {
     return {static_cast<const char*>(codes), static_cast<const char*>(scales), 128, (long)rows * 128, rows, 0};
 }
 
+constexpr int kMostParts = 64;
+
+TilePick pick_product(int M, int N, int K) { return tile_pick<mx4_t>(N, M, mx4_cols(K), kMostParts, device_cus()); }
 size_t product_bytes(int M, int N, int K) {
-    const int parts = tile_parts(N, M, mx4_cols(K) / kMxCols, device_cus());
+    const int parts = pick_product(M, N, K).parts;
     return parts > 1 ? part_bytes(N, M, parts) : 0;
 }
 
@@ -66,20 +69,20 @@ int product(unsigned flags, int M, int N, int K, const void* xc, const void* xs,
     g.M = N;
     g.N = M;
     g.K = mx4_cols(K);
-    const int parts = tile_parts(N, M, g.K / kMxCols, device_cus());
+    const TilePick pick = pick_product(M, N, K);
     const TileStore<T> store = {static_cast<T*>(y), N, static_cast<const T*>(bias), nullptr, (flags & WINO_FLAG_RELU) != 0};
-    if (parts == 1) {
-        tile_launch<mx4_t, K_INNER, K_INNER>(g, store, 1, s);
+    if (pick.parts == 1) {
+        tile_launch<mx4_t, K_INNER, K_INNER>(g, store, pick, M, s);
         LAUNCH_CHECK("mx4 product");
         return WINO_OK;
     }
-    const size_t need = part_bytes(N, M, parts);
+    const size_t need = part_bytes(N, M, pick.parts);
     if (!work || work_bytes < need) return fail(WINO_ERR_WORKSPACE, "mx4 product: workspace of %zu bytes, %zu needed", work ? work_bytes : 0, need);
     const long pitch = round_up(N, 4);
-    tile_launch<mx4_t, K_INNER, K_INNER>(g, TilePart{static_cast<float*>(work), pitch, 0}, parts, s);
+    tile_launch<mx4_t, K_INNER, K_INNER>(g, TilePart{static_cast<float*>(work), pitch, 0}, pick, M, s);
     LAUNCH_CHECK("mx4 product in parts");
     hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(N, 4) * M, 256)), dim3(256), 0, s,
-                       static_cast<const float*>(work), parts, pitch, N, M, store);
+                       static_cast<const float*>(work), pick.parts, pitch, N, M, store);
     LAUNCH_CHECK("mx4 join");
     return WINO_OK;
 }

@@ -98,7 +98,8 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
 
     // position in a k row (in pieces) that holds piece c; an involution
     static __device__ __forceinline__ int outer_swap(int krow, int c) {
-        return TileElem<T>::bytes == 4 ? c ^ (((krow >> 4) & 1) * 8) : c ^ ((krow & 3) * 4);
+        constexpr int inside = kRow / 16 - 1;                           // narrow tiles: as far as their rows reach
+        return TileElem<T>::bytes == 4 ? c ^ ((((krow >> 4) & 1) * 8) & inside) : c ^ (((krow & 3) * 4) & inside);
     }
     static __device__ __forceinline__ int inner_swap(int row) { return row & 7; }
 
@@ -109,7 +110,7 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
         if constexpr (!kOuter) {
             const int row = at >> 7;
             const int c = min((lane & 7) ^ inner_swap(row), k_left - 1);
-            return (unsigned)((long)min(row, op.rows - 1 - org) * op.pitch) + c * 16;
+            return (unsigned)((long)max(min(row, op.rows - 1 - org), 0) * op.pitch) + c * 16;
         } else {
             const int krow = at / kRow;
             const int org_piece = org / TileElem<T>::piece;
@@ -124,7 +125,8 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
     }
 
     __device__ __forceinline__ void init(const TileOperand& op, int org, int stage0, int wave, int lane) {
-        const uint64_t origin = kOuter ? (uint64_t)org * TileElem<T>::bytes : (uint64_t)org * (uint64_t)op.pitch;
+        // a tile may lie wholly behind the last row (an epilogue's cover): it then reads the last row
+        const uint64_t origin = kOuter ? (uint64_t)org * TileElem<T>::bytes : (uint64_t)min(org, op.rows - 1) * (uint64_t)op.pitch;
         base = uniform64((uint64_t)op.p + origin + (uint64_t)stage0 * (uint64_t)op.step);
         const int whole = kOuter ? 1 << 30 : 8;
 #pragma unroll
@@ -187,12 +189,14 @@ inline int tile_grid(int mt, int nt) { return (mt * nt + 7) / 8 * 8; }
 
 // WM x WN waves; a wave owns BM/WM x BN/WN of the tile.  RING stages of LDS, RING - 1 of them in flight.
 template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RING, class Epi>
-__global__ __launch_bounds__(64 * WM * WN, 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
+__global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
     constexpr int WAVES = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
     constexpr bool MX4 = std::is_same<T, mx4_t>::value;
     typedef TileSide<T, AO, BM, WAVES> SA;
     typedef TileSide<T, BO, BN, WAVES> SB;
-    constexpr int SC = MX4 ? (BM + BN) * 8 : 0;                        // scale bytes of a stage
+    // scale bytes of a stage: 8 per row, loaded 1 KB (128 rows) at a time
+    constexpr int SCA = (BM + 127) / 128, SCB = (BN + 127) / 128;
+    constexpr int SC = MX4 ? (SCA + SCB) * 1024 : 0;
     constexpr int SLOT = SA::kBytes + SB::kBytes + SC;
     __shared__ __align__(1024) char lds[RING * SLOT];
 
@@ -211,11 +215,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_gemm_kernel(TileArgs g, 
     sa.init(g.a, m0, first, wave, lane);
     sb.init(g.b, n0, first, wave, lane);
     const unsigned lds0 = lds_addr(lds);
-    // mx4: scale bytes as 16-byte pieces (two rows), BM/128 + BN/128 loads spread over the first waves
+    // mx4: scale bytes as 16-byte pieces (two rows), one load each by the first waves
     uint64_t sc_base = 0;
     unsigned sc_off = 0, sc_dst = 0;
     long sc_step = 0;
-    constexpr int SCA = BM / 128, SCB = BN / 128;
     static_assert(!MX4 || SCA + SCB <= WAVES, "a scale load per wave at most");
     if constexpr (MX4) {
         if (wave < SCA + SCB) {
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_gemm_kernel(TileArgs g, 
             sc_step = (long)rows2 * 16;
             sc_base = uniform64((uint64_t)op.scale + (uint64_t)first * (uint64_t)sc_step);
             sc_off = (unsigned)min(org / 2 + part * 64 + lane, rows2 - 1) * 16u;
-            sc_dst = SA::kBytes + SB::kBytes + (isa ? 0 : BM * 8) + part * 1024;
+            sc_dst = SA::kBytes + SB::kBytes + wave * 1024;
         }
     }
 
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_gemm_kernel(TileArgs g, 
 #pragma unroll
             for (int i = 0; i < MI; ++i) qa[i] = *reinterpret_cast<const unsigned*>(sca + ((wm * MI + i) * 32 + l32) * 8 + lh * 4);
 #pragma unroll
-            for (int n = 0; n < NI; ++n) qb[n] = *reinterpret_cast<const unsigned*>(sca + BM * 8 + ((wn * NI + n) * 32 + l32) * 8 + lh * 4);
+            for (int n = 0; n < NI; ++n) qb[n] = *reinterpret_cast<const unsigned*>(sca + SCA * 1024 + ((wn * NI + n) * 32 + l32) * 8 + lh * 4);
         }
         auto step = [&](auto jc) {
             constexpr int J = decltype(jc)::value;
@@ -302,22 +305,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_gemm_kernel(TileArgs g, 
         issue(s, fill);
         fill = fill + 1 == RING ? 0 : fill + 1;
     }
-    for (int s = first; s < last; ++s) {
-        // stage s has landed: the newer RING - 2 stages may still be in flight (fewer near the end)
+    // stage s has landed (the newer RING - 2 stages may still be in flight, fewer near the end) for every wave, and the
+    // slot before it is free: the stage RING - 1 ahead goes there
+    auto arrive = [&](int s) {
         asm volatile("" ::: "memory");
         if (RING > 2 && s + RING - 2 < last) wait_loads<(RING - 2) * (SA::kLoads + SB::kLoads)>();
         else wait_loads<0>();
-        __builtin_amdgcn_s_barrier();                                  // for every wave; and the slot before is free
+        __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
         if (s + RING - 1 < last) {
             issue(s + RING - 1, fill);
             fill = fill + 1 == RING ? 0 : fill + 1;
         }
-        if (ragged && s == last - 1) multiply(s, use, std::true_type{});
-        else multiply(s, use, std::false_type{});
+    };
+    const int whole = ragged ? last - 1 : last;
+    for (int s = first; s < whole; ++s) {
+        arrive(s);
+        multiply(s, use, std::false_type{});
         use = use + 1 == RING ? 0 : use + 1;
         __builtin_amdgcn_sched_barrier(0);
+    }
+    if (ragged) {
+        arrive(last - 1);
+        multiply(last - 1, use, std::true_type{});
     }
     wait_loads<0>();
     epi.template run<BM, BN, WM, WN, MI, NI>(acc, g, m0, n0, wm, wn, l32, lh, lds);
@@ -407,6 +418,21 @@ struct TilePart {
     }
 };
 
+// at[0] + at[plane] + ... in order, eight loads in flight
+template <typename V> __device__ __forceinline__ V sum_parts(const float* at, int parts, long plane) {
+    V s = {};
+    int z = 0;
+    for (; z + 8 <= parts; z += 8) {
+        V a[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) a[u] = *reinterpret_cast<const V*>(at + (z + u) * plane);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) s += a[u];
+    }
+    for (; z < parts; ++z) s += *reinterpret_cast<const V*>(at + z * plane);
+    return s;
+}
+
 // out[n][m] = relu?( scale * sum_z part[z][n][m] + bias[m] ): four m per thread, parts added in order
 template <typename T>
 __global__ __launch_bounds__(256) void tile_join_kernel(const float* __restrict__ part, int parts, long part_pitch, int M, int N,
@@ -416,9 +442,7 @@ __global__ __launch_bounds__(256) void tile_join_kernel(const float* __restrict_
     if (i >= (long)quads * N) return;
     const long row = i / quads;
     const int m = (int)(i - row * quads) * 4;
-    floatx4 s = {0.f, 0.f, 0.f, 0.f};
-    const float* at = part + row * part_pitch + m;
-    for (int z = 0; z < parts; ++z, at += (long)N * part_pitch) s += *reinterpret_cast<const floatx4*>(at);
+    const floatx4 s = sum_parts<floatx4>(part + row * part_pitch + m, parts, (long)N * part_pitch);
     const bool vec = o.pitch % 4 == 0 && (reinterpret_cast<uintptr_t>(o.out) & (4 * sizeof(T) - 1)) == 0;
     const float f = o.scale ? *o.scale : 1.f;
     float v[4];
@@ -436,25 +460,67 @@ constexpr int kTile = 128;               // edge of a tile
 
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-template <typename T, int AO, int BO, class Epi>
-inline void tile_launch(TileArgs g, const Epi& epi, int parts, hipStream_t s) {
-    g.mt = ceil_div(g.M, kTile);
-    g.nt = ceil_div(g.N, kTile);
+template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RING, class Epi>
+inline void tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hipStream_t s) {
+    g.mt = ceil_div(g.M, BM);
+    g.nt = ceil_div(cover, BN);
     g.stages = ceil_div(g.K, TileElem<T>::stage);
     g.split = ceil_div(g.stages, parts);
     parts = ceil_div(g.stages, g.split);
-    hipLaunchKernelGGL((tile_gemm_kernel<T, AO, BO, kTile, kTile, 2, 2, 2, Epi>), dim3(tile_grid(g.mt, g.nt), parts), dim3(256), 0, s, g, epi);
+    hipLaunchKernelGGL((tile_gemm_kernel<T, AO, BO, BM, BN, WM, WN, RING, Epi>), dim3(tile_grid(g.mt, g.nt), parts), dim3(64 * WM * WN), 0, s, g, epi);
 }
 
-// Into how many parts the reduction is cut: none while the tiles alone give every CU a workgroup, otherwise until two
-// workgroups per CU are there, each with two stages at least.
-inline int tile_parts(int M, int N, int stages, int cus) {
-    const long tiles = (long)ceil_div(M, kTile) * ceil_div(N, kTile);
-    if (tiles >= cus || stages < 4) return 1;
-    const int want = (int)std::min<long>(2L * cus / tiles, stages / 2);
-    const int split = ceil_div(stages, std::max(want, 1));
-    return ceil_div(stages, split);
+// How a product is cut: the tile (256 x 256, or 128 x cols) and the parts of its reduction.
+struct TilePick {
+    int big, cols, parts;
+    int edge() const { return big ? 256 : kTile; }      // m extent of a tile
+};
+
+// The cut with the smallest estimated time.  A CU works through its share of the (tile, part) items; an item takes the
+// longer of its multiplies and its operands' way into LDS; parts are written and read back once in fp32 by one more
+// launch.  `most` bounds the parts (1: the epilogue needs whole sums).  Rates in products / bytes per microsecond and CU,
+// fitted to the measured products of the classifier's sizes.
+template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, int cus) {
+    constexpr bool F32 = std::is_same<T, float>::value, MX4 = std::is_same<T, mx4_t>::value;
+    const double rate = F32 ? 0.28e6 : MX4 ? 6.5e6 : 2.1e6, rate_big = F32 ? 0.28e6 : MX4 ? 8.0e6 : 2.8e6, bytes = 45e3;
+    const int stages = ceil_div(K, TileElem<T>::stage);
+    TilePick best = {0, kTile, 1};
+    double least = 1e30;
+    for (int kind = 0; kind < 2; ++kind) {
+        const int cols = kind ? 256 : N <= 32 ? 32 : N <= 64 ? 64 : kTile, rows = kind ? 256 : kTile;
+        const long tiles = (long)ceil_div(M, rows) * ceil_div(N, cols);
+        if (kind && (M <= kTile || N <= kTile)) continue;
+        for (int parts = 1; parts <= most && parts <= std::max(1, stages / 2); parts += parts < 8 ? 1 : parts / 4) {
+            const int split = ceil_div(stages, parts);
+            if (ceil_div(stages, split) != parts) continue;
+            const long items = tiles * parts;
+            if (parts > 1 && (items > 4L * cus || (size_t)parts * M * N * 4 > (64u << 20))) break;
+            const double k = (double)split * TileElem<T>::stage;
+            const double mul = (double)rows * cols * k / (kind ? rate_big : rate);
+            const double move = (double)(rows + cols) * split * 128 / bytes;
+            // one small tile alone on its CU waits for its own loads
+            const double item = std::max(mul, move) * (!kind && items <= cus ? 1.25 : 1.0);
+            const double t = ceil_div(items, cus) * item + (parts > 1 ? 4.0 + (double)parts * M * N * 8 / 4e6 : 0.0);
+            if (t < least) {
+                least = t;
+                best = {kind, cols, parts};
+            }
+        }
+    }
+    return best;
 }
+
+// `cover`: rows of n that the epilogue has to reach (N or a little more)
+template <typename T, int AO, int BO, class Epi>
+inline void tile_launch(const TileArgs& g, const Epi& epi, const TilePick& pick, int cover, hipStream_t s) {
+    if (pick.big) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, 2>(g, epi, pick.parts, cover, s);
+    switch (pick.cols) {
+    case 32: return tile_launch_as<T, AO, BO, kTile, 32, 4, 1, std::is_same<T, mx4_t>::value ? 3 : 4>(g, epi, pick.parts, cover, s);
+    case 64: return tile_launch_as<T, AO, BO, kTile, 64, 4, 1, 3>(g, epi, pick.parts, cover, s);
+    default: return tile_launch_as<T, AO, BO, kTile, kTile, 2, 2, 2>(g, epi, pick.parts, cover, s);
+    }
+}
+
 inline size_t part_bytes(int M, int N, int parts) { return (size_t)parts * N * round_up(M, 4) * sizeof(float); }
 
 }  // namespace wino

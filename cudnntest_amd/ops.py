@@ -16,6 +16,7 @@ Two levels:
     sizes from them.
 """
 import enum
+import functools
 
 import torch
 
@@ -390,28 +391,37 @@ def layout_transform(t, src, dst):
 
 
 # ---- the network's head: 4-bit fully connected layers, softmax cross entropy ------------------
+# A call on a few rows takes a few microseconds on the GPU, so what the host does per call is kept short: sizes are
+# looked up by shape, and the device is switched only when it has to be.
 
-def _on(device, *tensors):
-    """Contiguous tensors of one GPU; None passes.  Their addresses."""
-    out = []
-    for t in tensors:
-        if t is None:
-            out.append(None)
-            continue
-        if t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}")
-        out.append(_ptr(t))
-    return out
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+
+
+def _address(t, device, what):
+    """Address of a contiguous tensor on `device` (a GPU); None passes."""
+    if t is None:
+        return None
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the first tensor on {device}")
+    return _ptr(t)
+
+
+def _call(device, fn, name, *args):
+    """One call into the library on `device`'s current stream."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index) if _raw_stream else _stream())
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _stream())
+    if rc:
+        _lib.check(rc, name)
 
 
 def _matrix(t, what):
     if t.dim() != 2:
         raise ValueError(f"{what} must be a matrix, got {t.dim()} dimensions")
     return t.shape
-
-
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _out_as(out, shape, dtype, device):
@@ -427,10 +437,25 @@ def _check_row_bias(bias, n, dtype):
         raise TypeError(f"bias must hold {n} elements of {dtype}")
 
 
+def mx4_geometry(rows, K):
+    import ctypes
+    kp, cb, sb = ctypes.c_int(), ctypes.c_size_t(), ctypes.c_size_t()
+    _lib.check(_lib.load().wino_mx4_geometry(rows, K, kp, cb, sb), "wino_mx4_geometry")
+    return dict(Kp=kp.value, code_bytes=cb.value, scale_bytes=sb.value)
+
+
+@functools.lru_cache(maxsize=4096)
+def _mx4_shapes(rows, K):
+    kb = mx4_geometry(rows, K)["Kp"] // 256
+    return (kb, rows, 128), (kb, (rows + 1) // 2 * 2, 8)
+
+
 class Mx4:
     """A matrix [rows][K] in microscaled 4-bit floating point (what wino_mx4_quantize writes): `codes`
     uint8 [Kp/256][rows][128], two elements a byte, and `scales` uint8 [Kp/256][rows rounded up to 2][8],
     one power-of-two exponent per 32 columns; Kp is K rounded up to 256."""
+
+    __slots__ = ("codes", "scales", "rows", "K")
 
     def __init__(self, codes, scales, rows, K):
         want = mx4_geometry(rows, K)
@@ -441,6 +466,15 @@ class Mx4:
                              f"scales, got {codes.numel()} and {scales.numel()}")
         self.codes, self.scales, self.rows, self.K = codes, scales, int(rows), int(K)
 
+    @classmethod
+    def _empty(cls, rows, K, device):
+        q = cls.__new__(cls)
+        codes, scales = _mx4_shapes(rows, K)
+        q.codes = torch.empty(codes, dtype=torch.uint8, device=device)
+        q.scales = torch.empty(scales, dtype=torch.uint8, device=device)
+        q.rows, q.K = rows, K
+        return q
+
     @property
     def shape(self):
         return (self.rows, self.K)
@@ -450,27 +484,17 @@ class Mx4:
         return self.codes.device
 
 
-def mx4_geometry(rows, K):
-    import ctypes
-    kp, cb, sb = ctypes.c_int(), ctypes.c_size_t(), ctypes.c_size_t()
-    _lib.check(_lib.load().wino_mx4_geometry(rows, K, kp, cb, sb), "wino_mx4_geometry")
-    return dict(Kp=kp.value, code_bytes=cb.value, scale_bytes=sb.value)
-
-
 def mx4_quantize(x, out=None):
     """x [rows][K] in microscaled 4 bits; `out` an Mx4 of the same shape to write into.  Asynchronous."""
     rows, K = _matrix(x, "x")
-    dt = _dt(x)
-    px, = _on(x.device, x)
+    dt, dev = _dt(x), x.device
+    px = _ptr(x)
     if out is None:
-        g = mx4_geometry(rows, K)
-        out = Mx4(torch.empty((g["Kp"] // 256, rows, 128), dtype=torch.uint8, device=x.device),
-                  torch.empty((g["Kp"] // 256, (rows + 1) // 2 * 2, 8), dtype=torch.uint8, device=x.device), rows, K)
+        out = Mx4._empty(rows, K, dev)
     elif out.shape != (rows, K):
         raise ValueError(f"out holds {out.shape}, x is {(rows, K)}")
-    pc, ps = _on(x.device, out.codes, out.scales)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().wino_mx4_quantize(dt, rows, K, px, pc, ps, _stream()), "wino_mx4_quantize")
+    _call(dev, _lib.load().wino_mx4_quantize, "wino_mx4_quantize", dt, rows, K, px, _address(out.codes, dev, "codes"),
+          _address(out.scales, dev, "scales"))
     return out
 
 
@@ -478,12 +502,17 @@ def mx4_dequantize(q, dtype=torch.float32, out=None):
     """The values that q's codes stand for, [rows][K] of `dtype`."""
     if dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {dtype}")
-    pc, ps = _on(q.device, q.codes, q.scales)
-    out = _out_as(out, q.shape, dtype, q.device)
-    po, = _on(q.device, out)
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.load().wino_mx4_dequantize(_DTYPES[dtype], q.rows, q.K, pc, ps, po, _stream()), "wino_mx4_dequantize")
+    dev = q.codes.device
+    out = _out_as(out, (q.rows, q.K), dtype, dev)
+    _call(dev, _lib.load().wino_mx4_dequantize, "wino_mx4_dequantize", _DTYPES[dtype], q.rows, q.K, _ptr(q.codes),
+          _address(q.scales, dev, "scales"), _address(out, dev, "out"))
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _mx4_workspace_bytes(M, N, K, device_index):
+    with torch.cuda.device(device_index):
+        return _lib.load().wino_mx4_workspace_bytes(M, N, K)
 
 
 def mx4_gemm(x, w, bias=None, relu=False, dtype=torch.float32, out=None):
@@ -492,15 +521,15 @@ def mx4_gemm(x, w, bias=None, relu=False, dtype=torch.float32, out=None):
         raise TypeError(f"unsupported dtype {dtype}")
     if x.K != w.K:
         raise ValueError(f"x has {x.K} columns, w has {w.K}")
-    M, N, K = x.rows, w.rows, w.K
+    M, N, K, dev = x.rows, w.rows, w.K, x.codes.device
     _check_row_bias(bias, N, dtype)
-    out = _out_as(out, (M, N), dtype, x.device)
-    xc, xs, wc, ws, pb, po = _on(x.device, x.codes, x.scales, w.codes, w.scales, bias, out)
-    with torch.cuda.device(x.device):
-        L = _lib.load()
-        work = _workspace(L.wino_mx4_workspace_bytes(M, N, K), x.device)
-        _lib.check(L.wino_mx4_gemm(_DTYPES[dtype], FLAG_RELU if relu else 0, M, N, K, xc, xs, wc, ws, pb, po,
-                                   work.data_ptr(), work.numel(), _stream()), "wino_mx4_gemm")
+    out = _out_as(out, (M, N), dtype, dev)
+    args = (_ptr(x.codes), _address(x.scales, dev, "x.scales"), _address(w.codes, dev, "w.codes"), _address(w.scales, dev, "w.scales"),
+            _address(bias, dev, "bias"), _address(out, dev, "out"))
+    nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(dev, _lib.load().wino_mx4_gemm, "wino_mx4_gemm", _DTYPES[dtype], FLAG_RELU if relu else 0, M, N, K, *args,
+          work.data_ptr(), nbytes)
     return out
 
 
@@ -510,15 +539,14 @@ def mx4_linear(x, w, bias=None, relu=False, out=None):
     M, K = _matrix(x, "x")
     if K != w.K:
         raise ValueError(f"x has {K} columns, w has {w.K}")
-    N, dt = w.rows, _dt(x)
+    N, dt, dev = w.rows, _dt(x), x.device
     _check_row_bias(bias, N, x.dtype)
-    out = _out_as(out, (M, N), x.dtype, x.device)
-    px, wc, ws, pb, po = _on(x.device, x, w.codes, w.scales, bias, out)
-    with torch.cuda.device(x.device):
-        L = _lib.load()
-        work = _workspace(L.wino_mx4_workspace_bytes(M, N, K), x.device)
-        _lib.check(L.wino_mx4_linear(dt, FLAG_RELU if relu else 0, M, N, K, px, wc, ws, pb, po, work.data_ptr(),
-                                     work.numel(), _stream()), "wino_mx4_linear")
+    out = _out_as(out, (M, N), x.dtype, dev)
+    args = (_ptr(x), _address(w.codes, dev, "w.codes"), _address(w.scales, dev, "w.scales"), _address(bias, dev, "bias"),
+            _address(out, dev, "out"))
+    nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _call(dev, _lib.load().wino_mx4_linear, "wino_mx4_linear", dt, FLAG_RELU if relu else 0, M, N, K, *args, work.data_ptr(), nbytes)
     return out
 
 
@@ -529,10 +557,22 @@ def _ce_arguments(x, w, target, bias):
         raise ValueError(f"x has {D} columns, w has {D2}")
     if w.dtype != x.dtype:
         raise TypeError("x and w must share a dtype")
-    if target.dtype != torch.int64 or tuple(target.shape) != (T,):
+    if target.dtype != torch.int64 or target.dim() != 1 or target.shape[0] != T:
         raise TypeError(f"target must be int64 of shape {(T,)}")
     _check_row_bias(bias, V, x.dtype)
     return T, D, V
+
+
+@functools.lru_cache(maxsize=4096)
+def _ce_workspace_bytes(dt, T, D, V, x_at, w_at, backward, device_index):
+    with torch.cuda.device(device_index):
+        return _lib.load().wino_linear_cross_entropy_workspace_bytes(dt, T, D, V, x_at, w_at, backward)
+
+
+def _ce_workspace(dt, T, D, V, px, pw, backward, dev):
+    # only the addresses' alignment matters
+    n = _ce_workspace_bytes(dt, T, D, V, 256 + px % 16, 256 + pw % 16, backward, dev.index)
+    return torch.empty(n, dtype=torch.uint8, device=dev), n
 
 
 def linear_cross_entropy(x, w, target, bias=None, ignore_index=-100):
@@ -541,14 +581,12 @@ def linear_cross_entropy(x, w, target, bias=None, ignore_index=-100):
     have loss 0, a target outside the classes gives NaN.  lse goes into linear_cross_entropy_backward.  Asynchronous."""
     T, D, V = _ce_arguments(x, w, target, bias)
     dt, dev = _dt(x), x.device
-    px, pw, pb, pt = _on(dev, x, w, bias, target)
-    loss, lse = torch.empty(2, T, dtype=torch.float32, device=dev).unbind(0)
-    with torch.cuda.device(dev):
-        L = _lib.load()
-        work = _workspace(L.wino_linear_cross_entropy_workspace_bytes(dt, T, D, V, px, pw, 0), dev)
-        _lib.check(L.wino_linear_cross_entropy(dt, T, D, V, px, pw, pb, pt, ignore_index, loss.data_ptr(), lse.data_ptr(),
-                                               work.data_ptr() if work is not None else None,
-                                               work.numel() if work is not None else 0, _stream()), "wino_linear_cross_entropy")
+    px, pw, pb, pt = _ptr(x), _address(w, dev, "w"), _address(bias, dev, "bias"), _address(target, dev, "target")
+    loss = torch.empty(T, dtype=torch.float32, device=dev)
+    lse = torch.empty(T, dtype=torch.float32, device=dev)
+    work, n = _ce_workspace(dt, T, D, V, px, pw, 0, dev)
+    _call(dev, _lib.load().wino_linear_cross_entropy, "wino_linear_cross_entropy", dt, T, D, V, px, pw, pb, pt, ignore_index,
+          loss.data_ptr(), lse.data_ptr(), work.data_ptr(), n)
     return loss, lse
 
 
@@ -558,19 +596,18 @@ def linear_cross_entropy_backward(grad, x, w, target, lse, bias=None, ignore_ind
     T, D, V = _ce_arguments(x, w, target, bias)
     dt, dev = _dt(x), x.device
     for t, name in ((grad, "grad"), (lse, "lse")):
-        if t.dtype != torch.float32 or tuple(t.shape) != (T,):
+        if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != T:
             raise TypeError(f"{name} must be float32 of shape {(T,)}")
-    px, pw, pb, pt, pg, pl = _on(dev, x, w, bias, target, grad, lse)
-    dx = torch.empty_like(x) if need[0] else None
-    dw = torch.empty_like(w) if need[1] else None
+    args = (_ptr(x), _address(w, dev, "w"), _address(bias, dev, "bias"), _address(target, dev, "target"))
+    pg, pl = _address(grad, dev, "grad"), _address(lse, dev, "lse")
+    dx = torch.empty((T, D), dtype=x.dtype, device=dev) if need[0] else None
+    dw = torch.empty((V, D), dtype=x.dtype, device=dev) if need[1] else None
     db = torch.empty(V, dtype=x.dtype, device=dev) if need[2] and bias is not None else None
     if dx is None and dw is None and db is None:
         return dx, dw, db
-    with torch.cuda.device(dev):
-        L = _lib.load()
-        work = _workspace(L.wino_linear_cross_entropy_workspace_bytes(dt, T, D, V, px, pw, 1), dev)
-        _lib.check(L.wino_linear_cross_entropy_backward(dt, T, D, V, px, pw, pb, pt, ignore_index, pg, pl, *_on(dev, dx, dw, db),
-                                                        work.data_ptr(), work.numel(), _stream()), "wino_linear_cross_entropy_backward")
+    work, n = _ce_workspace(dt, T, D, V, args[0], args[1], 1, dev)
+    _call(dev, _lib.load().wino_linear_cross_entropy_backward, "wino_linear_cross_entropy_backward", dt, T, D, V, *args, ignore_index,
+          pg, pl, *(None if t is None else t.data_ptr() for t in (dx, dw, db)), work.data_ptr(), n)
     return dx, dw, db
 
 
