@@ -101,7 +101,7 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
         constexpr int inside = kRow / 16 - 1;                           // narrow tiles: as far as their rows reach
         return TileElem<T>::bytes == 4 ? c ^ ((((krow >> 4) & 1) * 8) & inside) : c ^ (((krow & 3) * 4) & inside);
     }
-    static __device__ __forceinline__ int inner_swap(int row) { return row & 7; }
+    static __device__ __forceinline__ int inner_swap(int row) { return (row >> 1) & 7; }
 
     // byte offset, from the tile's origin in the stage at hand, of what this lane loads with load q of its wave;
     // k_left: k pieces (K_INNER) or k rows (K_OUTER) of the stage that exist
@@ -258,78 +258,104 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
             }
         }
     };
-    auto multiply = [&](int s, int slot, auto tail) {
-        constexpr bool TAIL = decltype(tail)::value;
+    // Two sets of fragments: while one step's are multiplied the next step's are on their way from LDS, across the stage
+    // border too.  The border sits before a stage's last multiplies: by then every wave holds the stage's last fragments,
+    // so its slot can be refilled, and the multiplies cover the barrier, the requests and the first reads of the next stage.
+    uintx4 fa[2][MI], fb[2][NI];
+    unsigned qa[2][MI] = {}, qb[2][NI] = {};
+    auto read = [&](int slot, auto jc) {
+        constexpr int J = decltype(jc)::value;
         const char* sta = lds + slot * SLOT;
         const char* stb = sta + SA::kBytes;
-        unsigned qa[MI] = {}, qb[NI] = {};
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[J & 1][i] = sa.fragment(sta, wm * MI + i, J, lane);
+#pragma unroll
+        for (int n = 0; n < NI; ++n) fb[J & 1][n] = sb.fragment(stb, wn * NI + n, J, lane);
+    };
+    auto read_scales = [&](int slot, int set) {
         if constexpr (MX4) {
-            const char* sca = stb + SB::kBytes;
+            const char* sca = lds + slot * SLOT + SA::kBytes + SB::kBytes;
 #pragma unroll
-            for (int i = 0; i < MI; ++i) qa[i] = *reinterpret_cast<const unsigned*>(sca + ((wm * MI + i) * 32 + l32) * 8 + lh * 4);
+            for (int i = 0; i < MI; ++i) qa[set][i] = *reinterpret_cast<const unsigned*>(sca + ((wm * MI + i) * 32 + l32) * 8 + lh * 4);
 #pragma unroll
-            for (int n = 0; n < NI; ++n) qb[n] = *reinterpret_cast<const unsigned*>(sca + SCA * 1024 + ((wn * NI + n) * 32 + l32) * 8 + lh * 4);
+            for (int n = 0; n < NI; ++n) qb[set][n] = *reinterpret_cast<const unsigned*>(sca + SCA * 1024 + ((wn * NI + n) * 32 + l32) * 8 + lh * 4);
         }
-        auto step = [&](auto jc) {
-            constexpr int J = decltype(jc)::value;
-            uintx4 fa[MI], fb[NI];
-#pragma unroll
-            for (int i = 0; i < MI; ++i) fa[i] = sa.fragment(sta, wm * MI + i, J, lane);
-#pragma unroll
-            for (int n = 0; n < NI; ++n) fb[n] = sb.fragment(stb, wn * NI + n, J, lane);
-            if constexpr (TAIL) {
-                // pieces past the end of the reduction: zero wherever k is inner (they were read from elsewhere in the
-                // row).  A k-outer operand needs no mask beside a k-inner one; where both are k-outer, the rows past
-                // the end exist and one of the two holds zeros in them.
-                const bool in = 4 * lh + J < (g.K - s * TileElem<T>::stage + TileElem<T>::piece - 1) / TileElem<T>::piece;
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-                    if (AO == K_INNER && !in) fa[i] = uintx4{0, 0, 0, 0};
-#pragma unroll
-                for (int n = 0; n < NI; ++n)
-                    if (BO == K_INNER && !in) fb[n] = uintx4{0, 0, 0, 0};
-            }
+    };
+    auto multiply = [&](int s, auto jc, auto tail) {
+        constexpr int J = decltype(jc)::value;
+        if constexpr (decltype(tail)::value && !MX4) {
+            // pieces past the end of the reduction: zero wherever k is inner (they were read from elsewhere in the
+            // row).  A k-outer operand needs no mask beside a k-inner one; where both are k-outer, the rows past
+            // the end exist and one of the two holds zeros in them.
+            const bool in = 4 * lh + J < (g.K - s * TileElem<T>::stage + TileElem<T>::piece - 1) / TileElem<T>::piece;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
+                if (AO == K_INNER && !in) fa[J & 1][i] = uintx4{0, 0, 0, 0};
 #pragma unroll
-                for (int n = 0; n < NI; ++n) tile_mma<T, J>(fa[i], fb[n], acc[i][n], qa[i], qb[n]);
-        };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
-        step(std::integral_constant<int, 2>{});
-        step(std::integral_constant<int, 3>{});
+            for (int n = 0; n < NI; ++n)
+                if (BO == K_INNER && !in) fb[J & 1][n] = uintx4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int n = 0; n < NI; ++n) tile_mma<T, J>(fa[J & 1][i], fb[J & 1][n], acc[i][n], qa[0][i], qb[0][n]);
     };
+    const std::integral_constant<int, 0> j0;
+    const std::integral_constant<int, 1> j1;
+    const std::integral_constant<int, 2> j2;
+    const std::integral_constant<int, 3> j3;
+    constexpr int LPW = SA::kLoads + SB::kLoads;
 
-    int fill = 0, use = 0;                                             // ring slots
-    for (int s = first; s < min(first + RING - 1, last); ++s) {
-        issue(s, fill);
-        fill = fill + 1 == RING ? 0 : fill + 1;
-    }
-    // stage s has landed (the newer RING - 2 stages may still be in flight, fewer near the end) for every wave, and the
-    // slot before it is free: the stage RING - 1 ahead goes there
-    auto arrive = [&](int s) {
+    const int ahead = min(first + RING, last);
+    for (int s = first; s < ahead; ++s) issue(s, s - first);
+    if (ahead - first == RING) wait_loads<(RING - 1) * LPW>();
+    else wait_loads<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0, j0);
+    read_scales(0, 0);
+    int slot = 0;
+    for (int s = first; s < last - 1; ++s) {
+        read(slot, j1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(s, j0, std::false_type{});
+        __builtin_amdgcn_sched_barrier(0);
+        read(slot, j2);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(s, j1, std::false_type{});
+        __builtin_amdgcn_sched_barrier(0);
+        read(slot, j3);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(s, j2, std::false_type{});
+        __builtin_amdgcn_sched_barrier(0);
+        // stage s + 1 has landed (the RING - 2 behind it may still be in flight, fewer near the end) and this wave has read
+        // all of stage s; behind the barrier that holds for every wave
         asm volatile("" ::: "memory");
-        if (RING > 2 && s + RING - 2 < last) wait_loads<(RING - 2) * (SA::kLoads + SB::kLoads)>();
+        if (RING > 2 && s + RING <= last) wait_loads<(RING - 2) * LPW>();
         else wait_loads<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        if (s + RING < last) issue(s + RING, slot);
+        slot = slot + 1 == RING ? 0 : slot + 1;
+        read(slot, j0);
+        read_scales(slot, 1);
         __builtin_amdgcn_sched_barrier(0);
-        if (s + RING - 1 < last) {
-            issue(s + RING - 1, fill);
-            fill = fill + 1 == RING ? 0 : fill + 1;
+        multiply(s, j3, std::false_type{});
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (MX4) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i) qa[0][i] = qa[1][i];
+#pragma unroll
+            for (int n = 0; n < NI; ++n) qb[0][n] = qb[1][n];
         }
-    };
-    const int whole = ragged ? last - 1 : last;
-    for (int s = first; s < whole; ++s) {
-        arrive(s);
-        multiply(s, use, std::false_type{});
-        use = use + 1 == RING ? 0 : use + 1;
-        __builtin_amdgcn_sched_barrier(0);
     }
-    if (ragged) {
-        arrive(last - 1);
-        multiply(last - 1, use, std::true_type{});
-    }
+    read(slot, j1);
+    multiply(last - 1, j0, std::true_type{});
+    read(slot, j2);
+    multiply(last - 1, j1, std::true_type{});
+    read(slot, j3);
+    multiply(last - 1, j2, std::true_type{});
+    multiply(last - 1, j3, std::true_type{});
     wait_loads<0>();
     epi.template run<BM, BN, WM, WN, MI, NI>(acc, g, m0, n0, wm, wn, l32, lh, lds);
 }
