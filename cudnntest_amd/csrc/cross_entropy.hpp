@@ -117,33 +117,29 @@ template <typename T> struct CeDl {
     long pitch;             // elements, a multiple of 8
     int row_end;
     template <int BM, int BN, int WM, int WN, int MI, int NI>
-    __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char*) const {
+    __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char* lds) const {
         const float f = scale ? *scale : 1.f;
+        float weight[NI], z[NI];
+        int hit[NI];
+        bool ignored[NI];
 #pragma unroll
         for (int n = 0; n < NI; ++n) {
             const int t = n0 + (wn * NI + n) * 32 + l32;
-            if (t >= row_end) continue;
             const bool in = t < g.N;
             const long long target = in ? rows.target[t] : rows.ignore;
-            const bool ignored = !in || target == rows.ignore;
-            const float weight = in ? row_weight(rows, target, grad[t]) * f : 0.f;
-            const float z = in ? lse[t] : 0.f;
-            const int hit = target >= v0 && target - v0 < g.M ? (int)(target - v0) : -1;
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int m = m0 + (wm * MI + i) * 32 + 8 * q + 4 * lh;
-                    if (m >= pitch) continue;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float b = bias && m + e < g.M ? to_f32(bias[m + e]) : 0.f;
-                        v[e] = m + e < g.M ? dl_of(acc[i][n][4 * q + e] + b, z, hit == m + e, weight, ignored) : 0.f;
-                    }
-                    store4<T>(dl + (long)t * pitch + m, v, 4, true);
-                }
+            ignored[n] = !in || target == rows.ignore;
+            weight[n] = in ? row_weight(rows, target, grad[t]) * f : 0.f;
+            z[n] = in ? lse[t] : 0.f;
+            hit[n] = target >= v0 && target - v0 < g.M ? (int)(target - v0) : -1;
         }
+        tile_store<T, WM, WN, MI, NI>(dl, pitch, m0, n0, row_end, (int)pitch, wm, wn, l32, lh, lds, false, [&](int i, int q, int n, float (&v)[4]) {
+            const int m = m0 + (wm * MI + i) * 32 + 8 * q + 4 * lh;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float b = bias && m + e < g.M ? to_f32(bias[m + e]) : 0.f;
+                v[e] = m + e < g.M ? dl_of(acc[i][n][4 * q + e] + b, z[n], hit[n] == m + e, weight[n], ignored[n]) : 0.f;
+            }
+        });
     }
 };
 
@@ -181,29 +177,45 @@ __global__ __launch_bounds__(256) static void ce_join_kernel(const float2* __res
     loss[t] = target == rows.ignore ? 0.f : target < 0 || target >= rows.V ? NAN : z - picked[t];
 }
 
-// the logit from the partial sums of a cut reduction
+// the partial sums of a cut reduction of the logits
 template <typename T> struct CeParts {
     const float* part;
     int parts;
     long pitch, plane;      // elements per row, per part
     const T* bias;
-    __device__ __forceinline__ float logit(long t, int v) const {
-        const float* at = part + t * pitch + v;
-        return sum_parts<float>(at, parts, plane) + (bias ? to_f32(bias[v]) : 0.f);
-    }
 };
 
-// small problems: loss and lse of one row per workgroup from the partial sums
+// small problems: loss and lse of one row per workgroup from the partial sums: 256 threads of four classes each, times
+// four quarters of the parts (up to 64 parts: a thread alone would wait for eight batches of loads one after the other)
 template <typename T>
-__global__ __launch_bounds__(256) void ce_rows_kernel(CeParts<T> p, CeRows rows, float* __restrict__ loss, float* __restrict__ lse) {
+__global__ __launch_bounds__(1024) void ce_rows_kernel(CeParts<T> p, CeRows rows, float* __restrict__ loss, float* __restrict__ lse) {
+    __shared__ floatx4 quarter[3][256];
     __shared__ float2 ex[256];
-    const int t = blockIdx.x;
+    __shared__ float picked;
+    const int t = blockIdx.x, c = threadIdx.x & 255, part = threadIdx.x >> 8;
+    const int per = (p.parts + 3) / 4, z0 = min(part * per, p.parts), z1 = min(z0 + per, p.parts);
+    const long long target = rows.target[t];
     float mx = -INFINITY, sum = 0.f;
-    for (int v = threadIdx.x; v < rows.V; v += 256) {
-        const float l = p.logit(t, v);
-        stats_join(mx, sum, l, l == -INFINITY ? 0.f : 1.f + (l - l));      // +inf and NaN make the row NaN
+    for (int v0 = 0; v0 < rows.V; v0 += 1024) {
+        const int v = v0 + 4 * c;
+        floatx4 s = {0.f, 0.f, 0.f, 0.f};
+        if (v < rows.V) s = sum_parts<floatx4>(p.part + t * p.pitch + v + z0 * p.plane, z1 - z0, p.plane);   // v + 3 < pitch
+        if (part) quarter[part - 1][c] = s;
+        __syncthreads();
+        if (part == 0) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) s += quarter[k][c];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (v + e >= rows.V) continue;
+                const float l = s[e] + (p.bias ? to_f32(p.bias[v + e]) : 0.f);
+                if (target == v + e) picked = l;
+                stats_join(mx, sum, l, l == -INFINITY ? 0.f : 1.f + (l - l));      // +inf and NaN make the row NaN
+            }
+        }
+        __syncthreads();
     }
-    ex[threadIdx.x] = make_float2(mx, sum);
+    if (part == 0) ex[c] = make_float2(mx, sum);
     __syncthreads();
     for (int k = 128; k > 0; k >>= 1) {
         if ((int)threadIdx.x < k) {
@@ -214,9 +226,8 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(CeParts<T> p, CeRows rows,
     }
     if (threadIdx.x != 0) return;
     const float z = mx + logf(sum);
-    const long long target = rows.target[t];
     lse[t] = z;
-    loss[t] = target == rows.ignore ? 0.f : target < 0 || target >= rows.V ? NAN : z - p.logit(t, (int)target);
+    loss[t] = target == rows.ignore ? 0.f : target < 0 || target >= rows.V ? NAN : z - picked;
 }
 
 // small problems: dl from the partial sums, four classes per thread
@@ -231,9 +242,14 @@ __global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int
     const bool ignored = !in || target == o.rows.ignore;
     const float weight = in ? row_weight(o.rows, target, o.grad[t]) * (o.scale ? *o.scale : 1.f) : 0.f;
     const float z = in ? o.lse[t] : 0.f;
+    floatx4 l = {0.f, 0.f, 0.f, 0.f};
+    if (in && m < o.rows.V) l = sum_parts<floatx4>(p.part + t * p.pitch + m, p.parts, p.plane);              // m + 3 < pitch of the parts
     float v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = in && m + e < o.rows.V ? dl_of(p.logit(t, m + e), z, target == m + e, weight, ignored) : 0.f;
+    for (int e = 0; e < 4; ++e) {
+        const float b = p.bias && m + e < o.rows.V ? to_f32(p.bias[m + e]) : 0.f;
+        v[e] = in && m + e < o.rows.V ? dl_of(l[e] + b, z, target == m + e, weight, ignored) : 0.f;
+    }
     store4<T>(o.dl + (long)t * o.pitch + m, v, 4, true);
 }
 

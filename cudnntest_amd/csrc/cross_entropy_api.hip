@@ -91,11 +91,11 @@ int check(const char* what, int dtype, int T, int D, int V, const void* x, const
 
 template <typename T> TileOperand inner(const T* p, long pitch, int rows) {
     const long b = pitch * (long)sizeof(T);
-    return {reinterpret_cast<const char*>(p), nullptr, b, 128, rows, 0};
+    return {reinterpret_cast<const char*>(p), nullptr, b, 0, rows, 0};
 }
 template <typename T> TileOperand outer(const T* p, long pitch, int k_rows) {
     const long b = pitch * (long)sizeof(T);
-    return {reinterpret_cast<const char*>(p), nullptr, b, b * TileElem<T>::stage, k_rows, (int)(b / 16)};
+    return {reinterpret_cast<const char*>(p), nullptr, b, 0, k_rows, (int)(b / 16)};
 }
 
 template <typename T> int pad_rows(const T* x, long rows, int cols, T* y, int pitch, hipStream_t s) {
@@ -153,7 +153,7 @@ template <typename T> struct Call {
         if (p.small) {
             CeParts<T> parts;
             if ((rc = partial_logits(&parts))) return rc;
-            hipLaunchKernelGGL((ce_rows_kernel<T>), dim3(T_), dim3(256), 0, s, parts, rows, loss, lse);
+            hipLaunchKernelGGL((ce_rows_kernel<T>), dim3(T_), dim3(1024), 0, s, parts, rows, loss, lse);
             LAUNCH_CHECK("ce_rows");
             return WINO_OK;
         }

@@ -7,9 +7,9 @@
 // that keeps the block's top binade on the grid, at the price of saturation between 6 and 8).  A block that holds a NaN or
 // an infinity gets b = 255, the format's NaN, so that it stays visible in every product.
 //
-// A quantised matrix of R rows and K columns is kept as the product kernels read it, Kp = K rounded up to 256:
-//     codes  [Kp/256][R][128]             two codes per byte, the lower column in the low half
-//     scales [Kp/256][R rounded up to 2][8]
+// A quantised matrix of R rows and K columns is kept as the product kernels read it, Kp = K rounded up to 128:
+//     codes  [Kp/128][R][64]              two codes per byte, the lower column in the low half
+//     scales [Kp/128][R rounded up to 4][4]
 // i.e. one stage of a tile's rows is one contiguous run.  Columns past K are zeros.
 #pragma once
 #include "common.hpp"
@@ -17,10 +17,10 @@
 
 namespace wino {
 
-constexpr int kMxCols = 256;             // columns of a stage
+constexpr int kMxCols = 128;             // columns of a stage
 inline int mx4_cols(int K) { return (int)round_up(K, kMxCols); }
 inline size_t mx4_code_bytes(long rows, int K) { return (size_t)rows * (mx4_cols(K) / 2); }
-inline size_t mx4_scale_bytes(long rows, int K) { return (size_t)round_up(rows, 2) * (mx4_cols(K) / 32); }
+inline size_t mx4_scale_bytes(long rows, int K) { return (size_t)round_up(rows, 4) * (mx4_cols(K) / 32); }
 
 // eight consecutive elements of a row as fp32; left: how many of them exist
 template <typename T> __device__ __forceinline__ void load8(const T* x, int left, bool vec, float (&v)[8]) {
@@ -62,12 +62,12 @@ __device__ __forceinline__ unsigned quad_max(unsigned v) {
     return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
 }
 
-// A workgroup takes 8 rows x 256 columns: a thread eight columns, four neighbouring threads a block.
+// A workgroup takes 16 rows x 128 columns: a thread eight columns, four neighbouring threads a block.
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__ x, int rows, int K, uint8_t* __restrict__ codes,
                                                            uint8_t* __restrict__ scales, int vec) {
     const unsigned kbs = (K + kMxCols - 1) / kMxCols;
-    const int row = blockIdx.x / kbs * 8 + (threadIdx.x >> 5), t = threadIdx.x & 31;
+    const int row = blockIdx.x / kbs * 16 + (threadIdx.x >> 4), t = threadIdx.x & 15;
     const int kb = blockIdx.x % kbs;
     if (row >= rows) return;
     const int k = kb * kMxCols + t * 8;
@@ -78,11 +78,12 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
     const unsigned b = mx4_scale_byte(quad_max(top));
     const unsigned c = b == 255 ? 0u : mx4_encode8(v, mx4_scale_value(b));
-    reinterpret_cast<unsigned*>(codes)[((long)kb * rows + row) * 32 + t] = c;
+    reinterpret_cast<unsigned*>(codes)[((long)kb * rows + row) * 16 + t] = c;
     if ((t & 3) == 0) {
-        uint8_t* s = scales + ((long)kb * ((rows + 1) & ~1) + row) * 8 + (t >> 2);
+        uint8_t* s = scales + ((long)kb * ((rows + 3) & ~3) + row) * 4 + (t >> 2);
         *s = (uint8_t)b;
-        if (row == rows - 1 && !(row & 1)) s[8] = 0;             // the row that pads an odd count
+        if (row == rows - 1)                                     // the rows that pad the count to four
+            for (int r = rows; r & 3; ++r) s[4 * (r - row)] = 0;
     }
 }
 
@@ -98,12 +99,12 @@ template <typename T>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                                                              int rows, int K, T* __restrict__ x, int vec) {
     const unsigned kbs = (K + kMxCols - 1) / kMxCols;
-    const int row = blockIdx.x / kbs * 8 + (threadIdx.x >> 5), t = threadIdx.x & 31;
+    const int row = blockIdx.x / kbs * 16 + (threadIdx.x >> 4), t = threadIdx.x & 15;
     const int kb = blockIdx.x % kbs;
     const int k = kb * kMxCols + t * 8;
     if (row >= rows || k >= K) return;
-    const unsigned c = reinterpret_cast<const unsigned*>(codes)[((long)kb * rows + row) * 32 + t];
-    const int b = scales[((long)kb * ((rows + 1) & ~1) + row) * 8 + (t >> 2)];
+    const unsigned c = reinterpret_cast<const unsigned*>(codes)[((long)kb * rows + row) * 16 + t];
+    const int b = scales[((long)kb * ((rows + 3) & ~3) + row) * 4 + (t >> 2)];
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = mx4_value(c >> (4 * e), b);

@@ -16,7 +16,7 @@ constexpr long kMaxTiles = 1L << 30;
 int check_shape(const char* what, long rows, int K) {
     if (rows <= 0 || K <= 0) return fail(WINO_ERR_INVALID, "%s: sizes must be positive (rows %ld, K %d)", what, rows, K);
     if (K > kMaxCols) return fail(WINO_ERR_UNSUPPORTED, "%s: K = %d, at most %d", what, K, kMaxCols);
-    if ((long)ceil_div(rows, 8) * (mx4_cols(K) / kMxCols) > kMaxTiles) return fail(WINO_ERR_UNSUPPORTED, "%s: %ld rows of %d", what, rows, K);
+    if ((long)ceil_div(rows, 16) * (mx4_cols(K) / kMxCols) > kMaxTiles) return fail(WINO_ERR_UNSUPPORTED, "%s: %ld rows of %d", what, rows, K);
     return WINO_OK;
 }
 int check_operand(const char* what, const void* codes, const void* scales) {
@@ -27,7 +27,7 @@ int check_operand(const char* what, const void* codes, const void* scales) {
 
 template <typename T> int quantize(int rows, int K, const void* x, void* codes, void* scales, hipStream_t s) {
     const int vec = !misaligned(x, 16) && (size_t)K * sizeof(T) % 16 == 0;
-    hipLaunchKernelGGL((mx4_quantize_kernel<T>), dim3(mx4_cols(K) / kMxCols * ceil_div(rows, 8)), dim3(256), 0, s,
+    hipLaunchKernelGGL((mx4_quantize_kernel<T>), dim3(mx4_cols(K) / kMxCols * ceil_div(rows, 16)), dim3(256), 0, s,
                        static_cast<const T*>(x), rows, K, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), vec);
     LAUNCH_CHECK("mx4_quantize");
     return WINO_OK;
@@ -40,14 +40,14 @@ int quantize_any(int dtype, int rows, int K, const void* x, void* codes, void* s
 
 template <typename T> int dequantize(int rows, int K, const void* codes, const void* scales, void* x, hipStream_t s) {
     const int vec = !misaligned(x, 16) && (size_t)K * sizeof(T) % 16 == 0;
-    hipLaunchKernelGGL((mx4_dequantize_kernel<T>), dim3(mx4_cols(K) / kMxCols * ceil_div(rows, 8)), dim3(256), 0, s,
+    hipLaunchKernelGGL((mx4_dequantize_kernel<T>), dim3(mx4_cols(K) / kMxCols * ceil_div(rows, 16)), dim3(256), 0, s,
                        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, K, static_cast<T*>(x), vec);
     LAUNCH_CHECK("mx4_dequantize");
     return WINO_OK;
 }
 
 TileOperand mx4_operand(const void* codes, const void* scales, int rows) {
-    return {static_cast<const char*>(codes), static_cast<const char*>(scales), 128, (long)rows * 128, rows, 0};
+    return {static_cast<const char*>(codes), static_cast<const char*>(scales), kMxCols / 2, 0, rows, 0};
 }
 
 constexpr int kMostParts = 64;

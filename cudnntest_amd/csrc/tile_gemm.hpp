@@ -23,6 +23,7 @@
 #pragma once
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "common.hpp"
 #include "mma.hpp"
@@ -37,15 +38,15 @@ struct mx4_t {};          // 32 values per 16-byte piece, with a power-of-two sc
 
 enum { K_INNER = 0, K_OUTER = 1 };
 
-// elements of k per 16-byte piece and per stage
-template <typename T> struct TileElem { static constexpr int piece = 16 / (int)sizeof(T), stage = 8 * piece, bytes = (int)sizeof(T); };
-template <> struct TileElem<mx4_t> { static constexpr int piece = 32, stage = 256, bytes = 0; };
+// elements of k per 16-byte piece
+template <typename T> struct TileElem { static constexpr int piece = 16 / (int)sizeof(T), bytes = (int)sizeof(T); };
+template <> struct TileElem<mx4_t> { static constexpr int piece = 32, bytes = 0; };
 
 struct TileOperand {
     const char* p;          // first byte of the operand
     const char* scale;      // mx4: [k stage][rows rounded up to 2][8] scale bytes
     long pitch;             // K_INNER: bytes from row to row; K_OUTER: bytes from one k row to the next
-    long step;              // bytes from stage to stage
+    long step;              // bytes from stage to stage (set by the launch)
     int rows;               // K_INNER: rows (m or n); K_OUTER: k rows that may be read
     int pieces;             // K_OUTER: 16-byte pieces per k row that may be read
 };
@@ -78,14 +79,19 @@ __device__ __forceinline__ void dma_piece(uint64_t sbase, unsigned off, unsigned
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(sbase) : "memory");
 }
 
+template <int... S, class F> __device__ __forceinline__ void for_each_step(std::integer_sequence<int, S...>, F&& f) {
+    (f(std::integral_constant<int, S>{}), ...);
+}
+
 template <int N> __device__ __forceinline__ void wait_loads() {      // at most N loads in flight, every LDS read returned
     static_assert(N < 64, "six bits of vmcnt");
     __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0x0 << 8) | ((N >> 4) << 14));
 }
 
 // One operand's side of a workgroup's tile: EXT rows (or columns) of it starting at org.
-template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
-    static constexpr int kBytes = EXT * 128;                           // of a stage in LDS, either order
+template <typename T, int ORDER, int EXT, int WAVES, int RB> struct TileSide {
+    static constexpr int kPieces = RB / 16, kSteps = kPieces / 2;      // of a row and stage, of a lane half
+    static constexpr int kBytes = EXT * RB;                            // of a stage in LDS, either order
     static constexpr int kLoads = kBytes / 1024 / WAVES;               // 1 KB loads per wave and stage
     static constexpr int kRow = EXT * TileElem<T>::bytes;              // K_OUTER: bytes of a k row in LDS
     static constexpr bool kOuter = ORDER == K_OUTER;
@@ -94,22 +100,23 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
 
     uint64_t base;            // of the stage to load next
     unsigned off[kLoads];
-    unsigned rd[4];           // K_INNER: a lane's LDS offsets of its pieces j = 0..3 (of 32-row block 0)
+    unsigned rd[kSteps];      // K_INNER: a lane's LDS offsets of its pieces j (of 32-row block 0)
 
     // position in a k row (in pieces) that holds piece c; an involution
     static __device__ __forceinline__ int outer_swap(int krow, int c) {
         constexpr int inside = kRow / 16 - 1;                           // narrow tiles: as far as their rows reach
-        return TileElem<T>::bytes == 4 ? c ^ ((((krow >> 4) & 1) * 8) & inside) : c ^ (((krow & 3) * 4) & inside);
+        return TileElem<T>::bytes == 4 ? c ^ ((krow / (4 * kSteps) & 1) * 8 & inside) : c ^ (((krow & 3) * 4) & inside);
     }
-    static __device__ __forceinline__ int inner_swap(int row) { return (row >> 1) & 7; }
+    // 16 neighbouring rows of one piece: spread over the 16 pieces of 256 bytes, a sweep of the banks
+    static __device__ __forceinline__ int inner_swap(int row) { return row / (16 / kPieces) & (kPieces - 1); }
 
     // byte offset, from the tile's origin in the stage at hand, of what this lane loads with load q of its wave;
     // k_left: k pieces (K_INNER) or k rows (K_OUTER) of the stage that exist
     static __device__ __forceinline__ unsigned source(const TileOperand& op, int org, int q, int wave, int lane, int k_left) {
         const int at = (wave * kLoads + q) * 1024 + lane * 16;
         if constexpr (!kOuter) {
-            const int row = at >> 7;
-            const int c = min((lane & 7) ^ inner_swap(row), k_left - 1);
+            const int row = at / RB;
+            const int c = min((lane % kPieces) ^ inner_swap(row), k_left - 1);
             return (unsigned)((long)max(min(row, op.rows - 1 - org), 0) * op.pitch) + c * 16;
         } else {
             const int krow = at / kRow;
@@ -120,7 +127,7 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
     }
     // what exists of a stage that starts at element k0 of the reduction
     static __device__ __forceinline__ int left(const TileOperand& op, int K, int k0) {
-        if constexpr (!kOuter) return min(8, (K - k0 + TileElem<T>::piece - 1) / TileElem<T>::piece);
+        if constexpr (!kOuter) return min(kPieces, (K - k0 + TileElem<T>::piece - 1) / TileElem<T>::piece);
         return op.rows - k0;
     }
 
@@ -128,19 +135,24 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
         // a tile may lie wholly behind the last row (an epilogue's cover): it then reads the last row
         const uint64_t origin = kOuter ? (uint64_t)org * TileElem<T>::bytes : (uint64_t)min(org, op.rows - 1) * (uint64_t)op.pitch;
         base = uniform64((uint64_t)op.p + origin + (uint64_t)stage0 * (uint64_t)op.step);
-        const int whole = kOuter ? 1 << 30 : 8;
+        const int whole = kOuter ? 1 << 30 : kPieces;
 #pragma unroll
         for (int q = 0; q < kLoads; ++q) off[q] = source(op, org, q, wave, lane, whole);
         if constexpr (!kOuter) {
             const int l32 = lane & 31, lh = lane >> 5;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) rd[j] = l32 * 128 + (((4 * lh + j) ^ inner_swap(l32)) << 4);
+            for (int j = 0; j < kSteps; ++j) rd[j] = l32 * RB + (((kSteps * lh + j) ^ inner_swap(l32)) << 4);
         }
     }
     __device__ __forceinline__ void load(const TileOperand& op, unsigned dst, int wave) {
 #pragma unroll
         for (int q = 0; q < kLoads; ++q) dma_piece(base, off[q], dst + (wave * kLoads + q) * 1024);
         base += (uint64_t)op.step;
+    }
+    template <int P, int OF> __device__ __forceinline__ void load_part(const TileOperand& op, unsigned dst, int wave) {
+#pragma unroll
+        for (int q = kLoads * P / OF; q < kLoads * (P + 1) / OF; ++q) dma_piece(base, off[q], dst + (wave * kLoads + q) * 1024);
+        if (P == OF - 1) base += (uint64_t)op.step;
     }
     // the last stage of a reduction that does not fill it
     __device__ __forceinline__ void load_tail(const TileOperand& op, int org, int k_left, unsigned dst, int wave, int lane) {
@@ -151,9 +163,9 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
     // piece j of block `blk` (32 rows or columns) for this lane
     __device__ __forceinline__ uintx4 fragment(const char* st, int blk, int j, int lane) const {
         if constexpr (!kOuter) {
-            return *reinterpret_cast<const uintx4*>(st + rd[j] + blk * 4096);
+            return *reinterpret_cast<const uintx4*>(st + rd[j] + blk * 32 * RB);
         } else if constexpr (TileElem<T>::bytes == 2) {
-            const int row = 8 * (4 * (lane >> 5) + j) + ((lane >> 2) & 3);            // row & 3 == (lane >> 2) & 3
+            const int row = 8 * (kSteps * (lane >> 5) + j) + ((lane >> 2) & 3);            // row & 3 == (lane >> 2) & 3
             const int piece = outer_swap(row, blk * 4 + ((lane >> 4) & 1) * 2) * 16 + (lane & 3) * 8;
             typedef __attribute__((address_space(3))) shortx4* ldsp;
             const char* at = st + row * kRow + piece;
@@ -163,7 +175,7 @@ template <typename T, int ORDER, int EXT, int WAVES> struct TileSide {
             const uintx2 l = __builtin_bit_cast(uintx2, lo), h = __builtin_bit_cast(uintx2, hi);
             return uintx4{l[0], l[1], h[0], h[1]};
         } else {
-            const int row = 4 * (4 * (lane >> 5) + j);
+            const int row = 4 * (kSteps * (lane >> 5) + j);
             const int col = outer_swap(row, blk * 8 + ((lane & 31) >> 2)) * 16 + (lane & 3) * 4;
             uintx4 v;
 #pragma unroll
@@ -188,14 +200,15 @@ __device__ __forceinline__ bool tile_of(int id, int mt, int nt, int& tm, int& tn
 inline int tile_grid(int mt, int nt) { return (mt * nt + 7) / 8 * 8; }
 
 // WM x WN waves; a wave owns BM/WM x BN/WN of the tile.  RING stages of LDS, RING - 1 of them in flight.
-template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RING, class Epi>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
+template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 || BM * BN * RB * RING > 128 * 128 * 128 * 2 ? 1 : 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
     constexpr int WAVES = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
     constexpr bool MX4 = std::is_same<T, mx4_t>::value;
-    typedef TileSide<T, AO, BM, WAVES> SA;
-    typedef TileSide<T, BO, BN, WAVES> SB;
-    // scale bytes of a stage: 8 per row, loaded 1 KB (128 rows) at a time
-    constexpr int SCA = (BM + 127) / 128, SCB = (BN + 127) / 128;
+    constexpr int STAGE = RB / 16 * TileElem<T>::piece, STEPS = RB / 32;   // elements of k, multiplies of a lane half
+    typedef TileSide<T, AO, BM, WAVES, RB> SA;
+    typedef TileSide<T, BO, BN, WAVES, RB> SB;
+    // scale bytes of a stage: one per piece, loaded 1 KB at a time
+    constexpr int SROW = RB / 16, SCA = (BM * SROW + 1023) / 1024, SCB = (BN * SROW + 1023) / 1024;
     constexpr int SC = MX4 ? (SCA + SCB) * 1024 : 0;
     constexpr int SLOT = SA::kBytes + SB::kBytes + SC;
     __shared__ __align__(1024) char lds[RING * SLOT];
@@ -208,14 +221,14 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     const int wm = wave / WN, wn = wave % WN;
     const int l32 = lane & 31, lh = lane >> 5;
     const int first = blockIdx.y * g.split, last = min(first + g.split, g.stages);
-    const bool ragged = last == g.stages && g.K % TileElem<T>::stage != 0;   // the last stage is a part of one
+    const bool ragged = last == g.stages && g.K % STAGE != 0;   // the last stage is a part of one
 
     SA sa;
     SB sb;
     sa.init(g.a, m0, first, wave, lane);
     sb.init(g.b, n0, first, wave, lane);
     const unsigned lds0 = lds_addr(lds);
-    // mx4: scale bytes as 16-byte pieces (two rows), one load each by the first waves
+    // mx4: scale bytes as 16-byte pieces (16 / SROW rows), one load each by the first waves
     uint64_t sc_base = 0;
     unsigned sc_off = 0, sc_dst = 0;
     long sc_step = 0;
@@ -225,10 +238,11 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
             const bool isa = wave < SCA;
             const TileOperand& op = isa ? g.a : g.b;
             const int part = isa ? wave : wave - SCA, org = isa ? m0 : n0;
-            const int rows2 = (op.rows + 1) >> 1;                                   // 16-byte pieces per stage
-            sc_step = (long)rows2 * 16;
+            constexpr int R = 16 / SROW;
+            const int rows16 = (op.rows + R - 1) / R;                               // 16-byte pieces per stage
+            sc_step = (long)rows16 * 16;
             sc_base = uniform64((uint64_t)op.scale + (uint64_t)first * (uint64_t)sc_step);
-            sc_off = (unsigned)min(org / 2 + part * 64 + lane, rows2 - 1) * 16u;
+            sc_off = (unsigned)min(org / R + part * 64 + lane, rows16 - 1) * 16u;
             sc_dst = SA::kBytes + SB::kBytes + wave * 1024;
         }
     }
@@ -244,7 +258,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     auto issue = [&](int s, int slot) {
         const unsigned dst = lds0 + slot * SLOT;
         if (ragged && s == last - 1) {
-            const int k0 = s * TileElem<T>::stage;
+            const int k0 = s * STAGE;
             sa.load_tail(g.a, m0, SA::left(g.a, g.K, k0), dst, wave, lane);
             sb.load_tail(g.b, n0, SB::left(g.b, g.K, k0), dst + SA::kBytes, wave, lane);
         } else {
@@ -274,11 +288,12 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     };
     auto read_scales = [&](int slot, int set) {
         if constexpr (MX4) {
+            typedef std::conditional_t<STEPS == 4, unsigned, unsigned short> SW;       // a lane's scale bytes of a stage
             const char* sca = lds + slot * SLOT + SA::kBytes + SB::kBytes;
 #pragma unroll
-            for (int i = 0; i < MI; ++i) qa[set][i] = *reinterpret_cast<const unsigned*>(sca + ((wm * MI + i) * 32 + l32) * 8 + lh * 4);
+            for (int i = 0; i < MI; ++i) qa[set][i] = *reinterpret_cast<const SW*>(sca + ((wm * MI + i) * 32 + l32) * SROW + lh * STEPS);
 #pragma unroll
-            for (int n = 0; n < NI; ++n) qb[set][n] = *reinterpret_cast<const unsigned*>(sca + SCA * 1024 + ((wn * NI + n) * 32 + l32) * 8 + lh * 4);
+            for (int n = 0; n < NI; ++n) qb[set][n] = *reinterpret_cast<const SW*>(sca + SCA * 1024 + ((wn * NI + n) * 32 + l32) * SROW + lh * STEPS);
         }
     };
     auto multiply = [&](int s, auto jc, auto tail) {
@@ -287,7 +302,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
             // pieces past the end of the reduction: zero wherever k is inner (they were read from elsewhere in the
             // row).  A k-outer operand needs no mask beside a k-inner one; where both are k-outer, the rows past
             // the end exist and one of the two holds zeros in them.
-            const bool in = 4 * lh + J < (g.K - s * TileElem<T>::stage + TileElem<T>::piece - 1) / TileElem<T>::piece;
+            const bool in = STEPS * lh + J < (g.K - s * STAGE + TileElem<T>::piece - 1) / TileElem<T>::piece;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
                 if (AO == K_INNER && !in) fa[J & 1][i] = uintx4{0, 0, 0, 0};
@@ -301,9 +316,32 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
             for (int n = 0; n < NI; ++n) tile_mma<T, J>(fa[J & 1][i], fb[J & 1][n], acc[i][n], qa[0][i], qb[0][n]);
     };
     const std::integral_constant<int, 0> j0;
-    const std::integral_constant<int, 1> j1;
-    const std::integral_constant<int, 2> j2;
-    const std::integral_constant<int, 3> j3;
+    const std::integral_constant<int, STEPS - 1> j_last;
+    // A full stage's requests, one share per step so that no step waits long for the CU's request path: with four steps A's
+    // in the first two and B's in the last two (16-bit 8192 x 4096 x 16384: 943 -> 902 us), with two all of them at once
+    // (4-bit: a split there gains nothing).
+    constexpr bool SPREAD = STEPS == 4;
+    bool pending = false;
+    int refill = 0;
+    auto share = [&](auto pc) {
+        constexpr int P = decltype(pc)::value;
+        const unsigned dst = lds0 + refill * SLOT;
+        if constexpr (P < 2) sa.template load_part<P, 2>(g.a, dst, wave);
+        else sb.template load_part<P - 2, 2>(g.b, dst + SA::kBytes, wave);
+    };
+    // steps 0 .. STEPS - 2 of stage s, each behind the request for the fragments of the next
+    auto all_but_last = [&](int s, int slot, auto tail) {
+        for_each_step(std::make_integer_sequence<int, STEPS - 1>{}, [&](auto jc) {
+            read(slot, std::integral_constant<int, decltype(jc)::value + 1>{});
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (SPREAD) {
+                if (pending) share(std::integral_constant<int, decltype(jc)::value + 1>{});
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            multiply(s, jc, tail);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    };
     constexpr int LPW = SA::kLoads + SB::kLoads;
 
     const int ahead = min(first + RING, last);
@@ -316,18 +354,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     read_scales(0, 0);
     int slot = 0;
     for (int s = first; s < last - 1; ++s) {
-        read(slot, j1);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(s, j0, std::false_type{});
-        __builtin_amdgcn_sched_barrier(0);
-        read(slot, j2);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(s, j1, std::false_type{});
-        __builtin_amdgcn_sched_barrier(0);
-        read(slot, j3);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(s, j2, std::false_type{});
-        __builtin_amdgcn_sched_barrier(0);
+        all_but_last(s, slot, std::false_type{});
         // stage s + 1 has landed (the RING - 2 behind it may still be in flight, fewer near the end) and this wave has read
         // all of stage s; behind the barrier that holds for every wave
         asm volatile("" ::: "memory");
@@ -335,12 +362,16 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
         else wait_loads<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + RING < last) issue(s + RING, slot);
+        refill = slot;
         slot = slot + 1 == RING ? 0 : slot + 1;
         read(slot, j0);
         read_scales(slot, 1);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(s, j3, std::false_type{});
+        pending = SPREAD && !MX4 && s + RING < (ragged ? last - 1 : last);      // (a partial stage goes in one piece)
+        if (pending) share(j0);
+        else if (s + RING < last) issue(s + RING, refill);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(s, j_last, std::false_type{});
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (MX4) {
 #pragma unroll
@@ -349,13 +380,8 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
             for (int n = 0; n < NI; ++n) qb[0][n] = qb[1][n];
         }
     }
-    read(slot, j1);
-    multiply(last - 1, j0, std::true_type{});
-    read(slot, j2);
-    multiply(last - 1, j1, std::true_type{});
-    read(slot, j3);
-    multiply(last - 1, j2, std::true_type{});
-    multiply(last - 1, j3, std::true_type{});
+    all_but_last(last - 1, slot, std::true_type{});
+    multiply(last - 1, j_last, std::true_type{});
     wait_loads<0>();
     epi.template run<BM, BN, WM, WN, MI, NI>(acc, g, m0, n0, wm, wn, l32, lh, lds);
 }
@@ -378,6 +404,73 @@ template <typename T> __device__ __forceinline__ void store4(T* y, const float (
         if (e < left) y[e] = from_f32<T>(v[e]);
 }
 
+// What a wave's accumulators become, written to out[n][m]: value(i, q, n, v) gives the four results at block i, quad q of
+// column block n.  A lane holds four of them per row, 8 or 16 bytes, which would touch 32 rows per store; so a wave turns
+// one 32-row block at a time in LDS of its own and stores rows in runs of MI * 32 elements, 16 bytes per lane (pieces
+// exchanged by row for the banks), or an element per lane where the output's rows are not 16-byte aligned.
+// rows past row_end and columns past col_end are not written; add: += (fp32).
+template <typename T, int WM, int WN, int MI, int NI, class F>
+__device__ __forceinline__ void tile_store(T* out, long pitch, int m0, int n0, int row_end, int col_end, int wm, int wn, int l32, int lh,
+                                           char* lds, bool add, F&& value) {
+    constexpr int CH = MI * 32 * (int)sizeof(T) / 16;                  // 16-byte pieces of a row of the block
+    const bool wide = (pitch * (long)sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    const int mb = m0 + wm * MI * 32;
+    __builtin_amdgcn_s_barrier();                                      // every wave is done with the last stage
+    asm volatile("" ::: "memory");
+    char* own = lds + (wm * WN + wn) * (32 * CH * 16);
+    auto swap = [](int row) { return CH >= 16 ? row & (CH - 1) : row / (16 / CH) & (CH - 1); };
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+        const int nb = n0 + (wn * NI + n) * 32;
+        if (nb >= row_end) continue;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float v[4];
+                value(i, q, n, v);
+                const int at = (i * 32 + 8 * q + 4 * lh) * (int)sizeof(T);
+                store4<T>(reinterpret_cast<T*>(own + l32 * CH * 16 + (((at >> 4) ^ swap(l32)) << 4) + (at & 15)), v, 4, true);
+            }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        if (wide) {
+#pragma unroll
+            for (int k = 0; k < CH / 2; ++k) {
+                const int idx = k * 64 + lh * 32 + l32, row = idx / CH, c = idx % CH;
+                const uintx4 v = *reinterpret_cast<const uintx4*>(own + row * CH * 16 + ((c ^ swap(row)) << 4));
+                constexpr int E = 16 / (int)sizeof(T);
+                const int m = mb + c * E;
+                if (nb + row >= row_end || m >= col_end) continue;
+                T* to = out + (long)(nb + row) * pitch + m;
+                if (m + E <= col_end) {
+                    if constexpr (sizeof(T) == 4) {
+                        floatx4 f = __builtin_bit_cast(floatx4, v);
+                        if (add) f += *reinterpret_cast<const floatx4*>(to);
+                        *reinterpret_cast<floatx4*>(to) = f;
+                    } else {
+                        *reinterpret_cast<uintx4*>(to) = v;
+                    }
+                } else {
+                    const Pack16<T> pk = __builtin_bit_cast(Pack16<T>, v);
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (m + e < col_end) to[e] = pk.e[e];
+                }
+            }
+        } else {
+            const int lane = lh * 32 + l32;
+            for (int k = 0; k < MI * 16; ++k) {
+                const int idx = k * 64 + lane, row = idx / (MI * 32), c = idx % (MI * 32), at = c * (int)sizeof(T);
+                const T v = *reinterpret_cast<const T*>(own + row * CH * 16 + (((at >> 4) ^ swap(row)) << 4) + (at & 15));
+                if (nb + row < row_end && mb + c < col_end) out[(long)(nb + row) * pitch + mb + c] = v;
+            }
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // out[n][m] = relu?( scale * acc + bias[m] ), rounded to T once
 template <typename T> struct TileStore {
     T* out;
@@ -386,34 +479,17 @@ template <typename T> struct TileStore {
     const float* scale;     // one factor in device memory, or null
     int relu;
     template <int BM, int BN, int WM, int WN, int MI, int NI>
-    __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char*) const {
-        const bool vec = pitch % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0;
+    __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char* lds) const {
         const float f = scale ? *scale : 1.f;
+        tile_store<T, WM, WN, MI, NI>(out, pitch, m0, n0, g.N, g.M, wm, wn, l32, lh, lds, false, [&](int i, int q, int n, float (&v)[4]) {
+            const int m = m0 + (wm * MI + i) * 32 + 8 * q + 4 * lh;
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int m = m0 + (wm * MI + i) * 32 + 8 * q + 4 * lh;
-                if (m >= g.M) continue;
-                float b[4] = {0.f, 0.f, 0.f, 0.f};
-                if (bias) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (m + e < g.M) b[e] = to_f32(bias[m + e]);
-                }
-#pragma unroll
-                for (int n = 0; n < NI; ++n) {
-                    const int row = n0 + (wn * NI + n) * 32 + l32;
-                    if (row >= g.N) continue;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        v[e] = acc[i][n][4 * q + e] * f + b[e];
-                        if (relu) v[e] = v[e] > 0.f || v[e] != v[e] ? v[e] : 0.f;      // a NaN stays one
-                    }
-                    store4<T>(out + row * pitch + m, v, g.M - m, vec);
-                }
+            for (int e = 0; e < 4; ++e) {
+                const float b = bias && m + e < g.M ? to_f32(bias[m + e]) : 0.f;
+                v[e] = acc[i][n][4 * q + e] * f + b;
+                if (relu) v[e] = v[e] > 0.f || v[e] != v[e] ? v[e] : 0.f;              // a NaN stays one
             }
+        });
     }
 };
 
@@ -423,24 +499,12 @@ struct TilePart {
     long pitch;             // elements, a multiple of 4; part is 16-byte aligned
     int add;
     template <int BM, int BN, int WM, int WN, int MI, int NI>
-    __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char*) const {
-        float* to = part + (long)blockIdx.y * g.N * pitch;
+    __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char* lds) const {
+        tile_store<float, WM, WN, MI, NI>(part + (long)blockIdx.y * g.N * pitch, pitch, m0, n0, g.N, (int)pitch, wm, wn, l32, lh, lds, add != 0,
+                                          [&](int i, int q, int n, float (&v)[4]) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int m = m0 + (wm * MI + i) * 32 + 8 * q + 4 * lh;
-                if (m >= g.M) continue;
-#pragma unroll
-                for (int n = 0; n < NI; ++n) {
-                    const int row = n0 + (wn * NI + n) * 32 + l32;
-                    if (row >= g.N) continue;
-                    floatx4* at = reinterpret_cast<floatx4*>(to + row * pitch + m);    // m + 3 < pitch
-                    floatx4 v = {acc[i][n][4 * q], acc[i][n][4 * q + 1], acc[i][n][4 * q + 2], acc[i][n][4 * q + 3]};
-                    if (add) v += *at;
-                    *at = v;
-                }
-            }
+                                              for (int e = 0; e < 4; ++e) v[e] = acc[i][n][4 * q + e];
+                                          });
     }
 };
 
@@ -486,19 +550,26 @@ constexpr int kTile = 128;               // edge of a tile
 
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RING, class Epi>
+template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
 inline void tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hipStream_t s) {
     g.mt = ceil_div(g.M, BM);
     g.nt = ceil_div(cover, BN);
-    g.stages = ceil_div(g.K, TileElem<T>::stage);
+    constexpr int stage = RB / 16 * TileElem<T>::piece;
+    const bool mx4 = std::is_same<T, mx4_t>::value;
+    g.a.step = mx4 ? g.a.rows * (long)RB : AO == K_INNER ? RB : g.a.pitch * stage;
+    g.b.step = mx4 ? g.b.rows * (long)RB : BO == K_INNER ? RB : g.b.pitch * stage;
+    g.stages = ceil_div(g.K, stage);
     g.split = ceil_div(g.stages, parts);
     parts = ceil_div(g.stages, g.split);
-    hipLaunchKernelGGL((tile_gemm_kernel<T, AO, BO, BM, BN, WM, WN, RING, Epi>), dim3(tile_grid(g.mt, g.nt), parts), dim3(64 * WM * WN), 0, s, g, epi);
+    hipLaunchKernelGGL((tile_gemm_kernel<T, AO, BO, BM, BN, WM, WN, RB, RING, Epi>), dim3(tile_grid(g.mt, g.nt), parts), dim3(64 * WM * WN), 0, s, g, epi);
 }
 
 // How a product is cut: the tile (256 x 256, or 128 x cols) and the parts of its reduction.
+template <typename T> constexpr int kStageOf = 8 * TileElem<T>::piece;     // elements of k in 128 bytes
+
 struct TilePick {
     int big, cols, parts;
+    int deep;                                           // twice the stages in flight, one workgroup to a CU
     int edge() const { return big ? 256 : kTile; }      // m extent of a tile
 };
 
@@ -509,11 +580,11 @@ struct TilePick {
 template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, int cus) {
     constexpr bool F32 = std::is_same<T, float>::value, MX4 = std::is_same<T, mx4_t>::value;
     const double rate = F32 ? 0.28e6 : MX4 ? 6.5e6 : 2.1e6, rate_big = F32 ? 0.28e6 : MX4 ? 8.0e6 : 2.8e6, bytes = 45e3;
-    const int stages = ceil_div(K, TileElem<T>::stage);
-    TilePick best = {0, kTile, 1};
+    const int stages = ceil_div(K, kStageOf<T>);
+    TilePick best = {0, kTile, 1, 0};
     double least = 1e30;
     for (int kind = 0; kind < 2; ++kind) {
-        const int cols = kind ? 256 : N <= 32 ? 32 : N <= 64 ? 64 : kTile, rows = kind ? 256 : kTile;
+        const int cols = kind ? 256 : N <= 32 && !MX4 ? 32 : N <= 64 ? 64 : kTile, rows = kind ? 256 : kTile;
         const long tiles = (long)ceil_div(M, rows) * ceil_div(N, cols);
         if (kind && (M <= kTile || N <= kTile)) continue;
         for (int parts = 1; parts <= most && parts <= std::max(1, stages / 2); parts += parts < 8 ? 1 : parts / 4) {
@@ -521,7 +592,7 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
             if (ceil_div(stages, split) != parts) continue;
             const long items = tiles * parts;
             if (parts > 1 && (items > 4L * cus || (size_t)parts * M * N * 4 > (64u << 20))) break;
-            const double k = (double)split * TileElem<T>::stage;
+            const double k = (double)split * kStageOf<T>;
             const double mul = (double)rows * cols * k / (kind ? rate_big : rate);
             const double move = (double)(rows + cols) * split * 128 / bytes;
             // one small tile alone on its CU waits for its own loads
@@ -529,7 +600,7 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
             const double t = ceil_div(items, cus) * item + (parts > 1 ? 4.0 + (double)parts * M * N * 8 / 4e6 : 0.0);
             if (t < least) {
                 least = t;
-                best = {kind, cols, parts};
+                best = {kind, cols, parts, !kind && cols == kTile && items <= cus};
             }
         }
     }
@@ -539,11 +610,15 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
 // `cover`: rows of n that the epilogue has to reach (N or a little more)
 template <typename T, int AO, int BO, class Epi>
 inline void tile_launch(const TileArgs& g, const Epi& epi, const TilePick& pick, int cover, hipStream_t s) {
-    if (pick.big) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, 2>(g, epi, pick.parts, cover, s);
+    constexpr int RB = std::is_same<T, mx4_t>::value ? 64 : 128;
+    if (pick.big) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
+    if constexpr (RB == 128)            // (a 4-bit stage of 32 rows is less than a load per wave)
+        if (pick.cols == 32) return tile_launch_as<T, AO, BO, kTile, 32, 4, 1, RB, 4>(g, epi, pick.parts, cover, s);
     switch (pick.cols) {
-    case 32: return tile_launch_as<T, AO, BO, kTile, 32, 4, 1, std::is_same<T, mx4_t>::value ? 3 : 4>(g, epi, pick.parts, cover, s);
-    case 64: return tile_launch_as<T, AO, BO, kTile, 64, 4, 1, 3>(g, epi, pick.parts, cover, s);
-    default: return tile_launch_as<T, AO, BO, kTile, kTile, 2, 2, 2>(g, epi, pick.parts, cover, s);
+    case 64: return tile_launch_as<T, AO, BO, kTile, 64, 4, 1, RB, RB == 64 ? 5 : 3>(g, epi, pick.parts, cover, s);
+    default:
+        if (pick.deep) return tile_launch_as<T, AO, BO, kTile, kTile, 2, 2, RB, RB == 64 ? 8 : 4>(g, epi, pick.parts, cover, s);
+        return tile_launch_as<T, AO, BO, kTile, kTile, 2, 2, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
     }
 }
 

@@ -446,14 +446,14 @@ def mx4_geometry(rows, K):
 
 @functools.lru_cache(maxsize=4096)
 def _mx4_shapes(rows, K):
-    kb = mx4_geometry(rows, K)["Kp"] // 256
-    return (kb, rows, 128), (kb, (rows + 1) // 2 * 2, 8)
+    kb = mx4_geometry(rows, K)["Kp"] // 128
+    return (kb, rows, 64), (kb, (rows + 3) // 4 * 4, 4)
 
 
 class Mx4:
     """A matrix [rows][K] in microscaled 4-bit floating point (what wino_mx4_quantize writes): `codes`
-    uint8 [Kp/256][rows][128], two elements a byte, and `scales` uint8 [Kp/256][rows rounded up to 2][8],
-    one power-of-two exponent per 32 columns; Kp is K rounded up to 256."""
+    uint8 [Kp/128][rows][64], two elements a byte, and `scales` uint8 [Kp/128][rows rounded up to 4][4],
+    one power-of-two exponent per 32 columns; Kp is K rounded up to 128."""
 
     __slots__ = ("codes", "scales", "rows", "K")
 

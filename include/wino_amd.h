@@ -327,9 +327,9 @@ int wino_stack_destroy(wino_stack_t *stack);
  * Microscaled 4-bit format (OCP MX, e2m1 elements): along a row, 32 values share a scale 2^(b - 127), b one byte; elements
  * are 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives.  A block with largest magnitude a gets b = clamp(floor(log2 a) + 125,
  * 0, 254) and elements round(x / scale), to nearest with ties to even, saturating at 6.  A block that holds a NaN or an
- * infinity gets b = 255 and stands for NaNs.  A matrix of `rows` x K, Kp = K rounded up to 256, is kept as
- *     codes  [Kp/256][rows][128]                      two elements per byte, the lower column in the low four bits
- *     scales [Kp/256][rows rounded up to 2][8]
+ * infinity gets b = 255 and stands for NaNs.  A matrix of `rows` x K, Kp = K rounded up to 128, is kept as
+ *     codes  [Kp/128][rows][64]                      two elements per byte, the lower column in the low four bits
+ *     scales [Kp/128][rows rounded up to 4][4]
  * with zeros in the columns past K.  Both must be 16-byte aligned. */
 int wino_mx4_geometry(int rows, int K, int *Kp, size_t *code_bytes, size_t *scale_bytes);
 /* x [rows][K] of `dtype` (a wino_dtype_t) to 4 bits, and the values that the codes stand for back to `dtype` (exact in

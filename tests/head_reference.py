@@ -16,9 +16,9 @@ def pow2(e):
 
 
 def mx4_encode(x):
-    """codes [rows][Kp], scale bytes [rows][Kp/32] of a matrix on the CPU, Kp a multiple of 256."""
+    """codes [rows][Kp], scale bytes [rows][Kp/32] of a matrix on the CPU, Kp a multiple of 128."""
     rows, K = x.shape
-    Kp = (K + 255) // 256 * 256
+    Kp = (K + 127) // 128 * 128
     v = torch.zeros(rows, Kp, dtype=torch.float64)
     v[:, :K] = x.double()
     b = v.view(rows, Kp // 32, 32)
@@ -41,9 +41,9 @@ def mx4_encode(x):
 def mx4_pack(codes, scales):
     """The library's operand layout."""
     rows, Kp = codes.shape
-    p = (codes[:, 0::2] | codes[:, 1::2] << 4).to(torch.uint8).view(rows, Kp // 256, 128).permute(1, 0, 2).contiguous()
-    s = torch.zeros(Kp // 256, (rows + 1) // 2 * 2, 8, dtype=torch.uint8)
-    s[:, :rows] = scales.to(torch.uint8).view(rows, Kp // 256, 8).permute(1, 0, 2)
+    p = (codes[:, 0::2] | codes[:, 1::2] << 4).to(torch.uint8).view(rows, Kp // 128, 64).permute(1, 0, 2).contiguous()
+    s = torch.zeros(Kp // 128, (rows + 3) // 4 * 4, 4, dtype=torch.uint8)
+    s[:, :rows] = scales.to(torch.uint8).view(rows, Kp // 128, 4).permute(1, 0, 2)
     return p, s
 
 

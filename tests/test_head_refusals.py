@@ -13,8 +13,8 @@ OFF8 = ctypes.c_void_p(264)
 
 
 def test_mx4_geometry():
-    assert ops.mx4_geometry(3, 257) == dict(Kp=512, code_bytes=3 * 256, scale_bytes=4 * 16)
-    assert ops.mx4_geometry(1, 1) == dict(Kp=256, code_bytes=128, scale_bytes=16)
+    assert ops.mx4_geometry(3, 257) == dict(Kp=384, code_bytes=3 * 192, scale_bytes=4 * 12)
+    assert ops.mx4_geometry(1, 1) == dict(Kp=128, code_bytes=64, scale_bytes=16)
     L = _lib.load()
     assert L.wino_mx4_geometry(0, 5, None, None, None) == INVALID
     assert L.wino_mx4_geometry(5, -1, None, None, None) == INVALID
@@ -99,7 +99,7 @@ def test_python_layer_refuses():
         ops.mx4_quantize(torch.zeros(4))
     with pytest.raises(TypeError):
         ops.mx4_quantize(x.double())
-    q = ops.Mx4(torch.zeros(1, 4, 128, dtype=torch.uint8), torch.zeros(1, 4, 8, dtype=torch.uint8), 4, 32)
+    q = ops.Mx4(torch.zeros(1, 4, 64, dtype=torch.uint8), torch.zeros(1, 4, 4, dtype=torch.uint8), 4, 32)
     with pytest.raises(ValueError):
         ops.Mx4(q.codes, q.scales, 4, 257)
     with pytest.raises(TypeError):
