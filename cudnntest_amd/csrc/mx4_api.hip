@@ -16,7 +16,7 @@ constexpr long kMaxTiles = 1L << 30;
 int check_shape(const char* what, long rows, int K) {
     if (rows <= 0 || K <= 0) return fail(WINO_ERR_INVALID, "%s: sizes must be positive (rows %ld, K %d)", what, rows, K);
     if (K > kMaxCols) return fail(WINO_ERR_UNSUPPORTED, "%s: K = %d, at most %d", what, K, kMaxCols);
-    if ((long)ceil_div(rows, 16) * (mx4_cols(K) / kMxCols) > kMaxTiles) return fail(WINO_ERR_UNSUPPORTED, "%s: %ld rows of %d", what, rows, K);
+    if (mx4_grid<float>(rows, K) > kMaxTiles) return fail(WINO_ERR_UNSUPPORTED, "%s: %ld rows of %d", what, rows, K);
     return WINO_OK;
 }
 int check_operand(const char* what, const void* codes, const void* scales) {
@@ -27,7 +27,7 @@ int check_operand(const char* what, const void* codes, const void* scales) {
 
 template <typename T> int quantize(int rows, int K, const void* x, void* codes, void* scales, hipStream_t s) {
     const int vec = !misaligned(x, 16) && (size_t)K * sizeof(T) % 16 == 0;
-    hipLaunchKernelGGL((mx4_quantize_kernel<T>), dim3(mx4_cols(K) / kMxCols * ceil_div(rows, 16)), dim3(256), 0, s,
+    hipLaunchKernelGGL((mx4_quantize_kernel<T>), dim3(mx4_grid<T>(rows, K)), dim3(256), 0, s,
                        static_cast<const T*>(x), rows, K, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), vec);
     LAUNCH_CHECK("mx4_quantize");
     return WINO_OK;
@@ -40,7 +40,7 @@ int quantize_any(int dtype, int rows, int K, const void* x, void* codes, void* s
 
 template <typename T> int dequantize(int rows, int K, const void* codes, const void* scales, void* x, hipStream_t s) {
     const int vec = !misaligned(x, 16) && (size_t)K * sizeof(T) % 16 == 0;
-    hipLaunchKernelGGL((mx4_dequantize_kernel<T>), dim3(mx4_cols(K) / kMxCols * ceil_div(rows, 16)), dim3(256), 0, s,
+    hipLaunchKernelGGL((mx4_dequantize_kernel<T>), dim3(mx4_grid<T>(rows, K)), dim3(256), 0, s,
                        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), rows, K, static_cast<T*>(x), vec);
     LAUNCH_CHECK("mx4_dequantize");
     return WINO_OK;
@@ -53,7 +53,39 @@ TileOperand mx4_operand(const void* codes, const void* scales, int rows) {
 constexpr int kMostParts = 64;
 
 TilePick pick_product(int M, int N, int K) { return tile_pick<mx4_t>(N, M, mx4_cols(K), kMostParts, device_cus()); }
+// Up to 16 rows always (one column block of the multiply), up to 32 while the reduction is short: 32 x 1000 x 4096 takes
+// 5.0 us against 7.3 through the tiles, 32 x 4096 x 25088 20.8 us against 15.3 -- x's codes are then read by every
+// workgroup in as many bytes as w's.
+bool few_rows(int M, int K) { return M <= 16 || (M <= kFewRows && K <= 8192); }
+bool few_quant(int M, int K) { return few_rows(M, K) && (long)M * mx4_cols(K) <= kFewQuant; }
+
+// x (in T) or its codes, whichever is not null
+template <typename T>
+int few_rows_product(unsigned flags, int M, int N, int K, const void* x, const void* xc, const void* xs, const void* wc, const void* ws,
+                     const void* bias, void* y, hipStream_t s) {
+    const int waves = std::min(kFewWaves, std::max(4, mx4_cols(K) / kMxCols));
+    const int vec = x && !misaligned(x, 16) && (size_t)K * sizeof(T) % 16 == 0;
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(ceil_div(N, 16)), dim3(64 * waves), 0, s, static_cast<const T*>(x), static_cast<const uint8_t*>(xc),
+                           static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(wc), static_cast<const uint8_t*>(ws),
+                           static_cast<const T*>(bias), static_cast<T*>(y), M, N, K, (flags & WINO_FLAG_RELU) != 0, vec);
+    };
+    if (x && M <= 16) launch(mx4_few_rows_kernel<T, 1, true>);
+    else if (x) launch(mx4_few_rows_kernel<T, 2, true>);
+    else if (M <= 16) launch(mx4_few_rows_kernel<T, 1, false>);
+    else launch(mx4_few_rows_kernel<T, 2, false>);
+    LAUNCH_CHECK("mx4 product of few rows");
+    return WINO_OK;
+}
+int few_rows_any(int dtype, unsigned flags, int M, int N, int K, const void* x, const void* xc, const void* xs, const void* wc,
+                 const void* ws, const void* bias, void* y, hipStream_t s) {
+    return dtype == WINO_F32   ? few_rows_product<float>(flags, M, N, K, x, xc, xs, wc, ws, bias, y, s)
+           : dtype == WINO_F16 ? few_rows_product<f16_t>(flags, M, N, K, x, xc, xs, wc, ws, bias, y, s)
+                               : few_rows_product<bf16_t>(flags, M, N, K, x, xc, xs, wc, ws, bias, y, s);
+}
+
 size_t product_bytes(int M, int N, int K) {
+    if (few_rows(M, K)) return 0;
     const int parts = pick_product(M, N, K).parts;
     return parts > 1 ? part_bytes(N, M, parts) : 0;
 }
@@ -88,6 +120,7 @@ int product(unsigned flags, int M, int N, int K, const void* xc, const void* xs,
 }
 int product_any(int dtype, unsigned flags, int M, int N, int K, const void* xc, const void* xs, const void* wc, const void* ws,
                 const void* bias, void* y, void* work, size_t work_bytes, hipStream_t s) {
+    if (few_rows(M, K)) return few_rows_any(dtype, flags, M, N, K, nullptr, xc, xs, wc, ws, bias, y, s);
     return dtype == WINO_F32   ? product<float>(flags, M, N, K, xc, xs, wc, ws, bias, y, work, work_bytes, s)
            : dtype == WINO_F16 ? product<f16_t>(flags, M, N, K, xc, xs, wc, ws, bias, y, work, work_bytes, s)
                                : product<bf16_t>(flags, M, N, K, xc, xs, wc, ws, bias, y, work, work_bytes, s);
@@ -147,6 +180,7 @@ int wino_mx4_dequantize(int dtype, int rows, int K, const void* codes, const voi
 
 size_t wino_mx4_workspace_bytes(int M, int N, int K) {
     if (check_shape("wino_mx4_workspace_bytes", M, K) || check_shape("wino_mx4_workspace_bytes", N, K)) return 0;
+    if (few_quant(M, K)) return 0;
     return round_up(mx4_code_bytes(M, K), 256) + round_up(mx4_scale_bytes(M, K), 256) + round_up(product_bytes(M, N, K), 256);
 }
 
@@ -164,6 +198,7 @@ int wino_mx4_linear(int dtype, unsigned flags, int M, int N, int K, const void* 
     if (rc) return rc;
     if (!x) return fail(WINO_ERR_INVALID, "wino_mx4_linear: null input");
     if (misaligned(x, dtype_size(dtype))) return fail(WINO_ERR_INVALID, "wino_mx4_linear: x must be aligned to its element type");
+    if (few_quant(M, K)) return few_rows_any(dtype, flags, M, N, K, x, nullptr, nullptr, wcodes, wscales, bias, y, (hipStream_t)stream);
     const size_t need = wino_mx4_workspace_bytes(M, N, K);
     if (!workspace || workspace_bytes < need)
         return fail(WINO_ERR_WORKSPACE, "wino_mx4_linear: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);

@@ -583,24 +583,25 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
     const int stages = ceil_div(K, kStageOf<T>);
     TilePick best = {0, kTile, 1, 0};
     double least = 1e30;
-    for (int kind = 0; kind < 2; ++kind) {
-        const int cols = kind ? 256 : N <= 32 && !MX4 ? 32 : N <= 64 ? 64 : kTile, rows = kind ? 256 : kTile;
+    for (int kind = 0; kind < 3; ++kind) {                              // 128 x cols, 256 x 256, 128 x 64 for many rows
+        const int few = N <= 32 && !MX4 ? 32 : N <= 64 ? 64 : kTile;
+        if ((kind == 1 && (M <= kTile || N <= kTile)) || (kind == 2 && (!F32 || few < kTile))) continue;
+        const int cols = kind == 1 ? 256 : kind == 2 ? 64 : few, rows = kind == 1 ? 256 : kTile;
         const long tiles = (long)ceil_div(M, rows) * ceil_div(N, cols);
-        if (kind && (M <= kTile || N <= kTile)) continue;
         for (int parts = 1; parts <= most && parts <= std::max(1, stages / 2); parts += parts < 8 ? 1 : parts / 4) {
             const int split = ceil_div(stages, parts);
             if (ceil_div(stages, split) != parts) continue;
             const long items = tiles * parts;
             if (parts > 1 && (items > 4L * cus || (size_t)parts * M * N * 4 > (64u << 20))) break;
             const double k = (double)split * kStageOf<T>;
-            const double mul = (double)rows * cols * k / (kind ? rate_big : rate);
+            const double mul = (double)rows * cols * k / (kind == 1 ? rate_big : kind == 2 ? 0.88 * rate : rate);
             const double move = (double)(rows + cols) * split * 128 / bytes;
             // one small tile alone on its CU waits for its own loads
-            const double item = std::max(mul, move) * (!kind && items <= cus ? 1.25 : 1.0);
+            const double item = std::max(mul, move) * (kind != 1 && items <= cus ? 1.25 : 1.0);
             const double t = ceil_div(items, cus) * item + (parts > 1 ? 4.0 + (double)parts * M * N * 8 / 4e6 : 0.0);
             if (t < least) {
                 least = t;
-                best = {kind, cols, parts, !kind && cols == kTile && items <= cus};
+                best = {kind == 1, cols, parts, !kind && cols == kTile && items <= cus};
             }
         }
     }

@@ -527,9 +527,9 @@ def mx4_gemm(x, w, bias=None, relu=False, dtype=torch.float32, out=None):
     args = (_ptr(x.codes), _address(x.scales, dev, "x.scales"), _address(w.codes, dev, "w.codes"), _address(w.scales, dev, "w.scales"),
             _address(bias, dev, "bias"), _address(out, dev, "out"))
     nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev).data_ptr() if nbytes else None
     _call(dev, _lib.load().wino_mx4_gemm, "wino_mx4_gemm", _DTYPES[dtype], FLAG_RELU if relu else 0, M, N, K, *args,
-          work.data_ptr(), nbytes)
+          work, nbytes)
     return out
 
 
@@ -545,8 +545,8 @@ def mx4_linear(x, w, bias=None, relu=False, out=None):
     args = (_ptr(x), _address(w.codes, dev, "w.codes"), _address(w.scales, dev, "w.scales"), _address(bias, dev, "bias"),
             _address(out, dev, "out"))
     nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call(dev, _lib.load().wino_mx4_linear, "wino_mx4_linear", dt, FLAG_RELU if relu else 0, M, N, K, *args, work.data_ptr(), nbytes)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev).data_ptr() if nbytes else None
+    _call(dev, _lib.load().wino_mx4_linear, "wino_mx4_linear", dt, FLAG_RELU if relu else 0, M, N, K, *args, work, nbytes)
     return out
 
 

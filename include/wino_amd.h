@@ -336,7 +336,8 @@ int wino_mx4_geometry(int rows, int K, int *Kp, size_t *code_bytes, size_t *scal
  * fp32 and bf16; in f16 values below its range are rounded, values above it become infinite) */
 int wino_mx4_quantize(int dtype, int rows, int K, const void *x, void *codes, void *scales, void *stream);
 int wino_mx4_dequantize(int dtype, int rows, int K, const void *codes, const void *scales, void *x, void *stream);
-/* bytes of workspace that wino_mx4_gemm and wino_mx4_linear need for these sizes (0 for invalid ones); 256-byte aligned */
+/* bytes of workspace that wino_mx4_gemm and wino_mx4_linear need for these sizes (0 for invalid ones, and for few rows,
+ * which need none: the pointer may then be NULL); 256-byte aligned */
 size_t wino_mx4_workspace_bytes(int M, int N, int K);
 /* y[m][n] = relu?( sum_k x[m][k] w[n][k] + bias[n] ): both matrices quantised; products of 4-bit values are exact, sums are
  * fp32, y and bias (N elements or NULL) are of `dtype`.  flags: 0 or WINO_FLAG_RELU. */

@@ -32,7 +32,8 @@ def test_mx4_refusals():
     assert L.wino_mx4_dequantize(0, 1, 32, P, P, None, None) == INVALID
     assert L.wino_mx4_dequantize(0, 1, 32, P, OFF8, P, None) == INVALID
     assert L.wino_mx4_workspace_bytes(0, 1, 1) == 0
-    need = L.wino_mx4_workspace_bytes(4, 8, 32)
+    assert L.wino_mx4_workspace_bytes(4, 8, 32) == 0        # few rows need none
+    need = L.wino_mx4_workspace_bytes(40, 8, 32)
     assert need > 0
     gemm = lambda **k: L.wino_mx4_gemm(*[k.get(n, d) for n, d in (
         ("dtype", 0), ("flags", 0), ("M", 4), ("N", 8), ("K", 32), ("xc", P), ("xs", P), ("wc", P), ("ws", P), ("bias", P), ("y", P), ("work", P),
@@ -49,7 +50,7 @@ def test_mx4_refusals():
     assert gemm(y=ODD) == INVALID
     assert gemm(bias=ODD) == INVALID
     assert gemm(work=OFF8) == INVALID
-    lin = lambda x, work, nbytes: L.wino_mx4_linear(0, 0, 4, 8, 32, x, P, P, None, P, work, nbytes, None)
+    lin = lambda x, work, nbytes: L.wino_mx4_linear(0, 0, 40, 8, 32, x, P, P, None, P, work, nbytes, None)
     assert lin(None, P, need) == INVALID
     assert lin(ODD, P, need) == INVALID
     assert lin(P, None, need) == WORKSPACE
