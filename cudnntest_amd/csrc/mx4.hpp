@@ -64,8 +64,12 @@ __device__ __forceinline__ unsigned quad_max(unsigned v) {
 
 // Both conversions move 16 bytes of the wide side per lane, so that a wave's access is one run of 1 KB per two rows (fp32)
 // or four: E = 4 or 8 columns, 32 / E neighbouring lanes to a block.  A workgroup takes kMxStages stages of 128 columns
-// of 8 or 16 rows, all of a thread's loads in flight before the first is used.
-constexpr int kMxStages = 4;
+// of 8 or 16 rows, all of a thread's loads in flight before the first is used (4096 x 25088 fp32, 1 / 2 / 4 stages: quantise
+// 91 / 81 / 77 us, one row of 4096 2.9 / 3.1 / 3.4 us).  The wide side is read or written past the caches' replacement order
+// (non-temporal): always when it is written (the same matrix 128 -> 66 us, 4096 x 8192 bf16 17.7 -> 15.7: 7 TB/s), when it is
+// read only if it could not have been in the 256 MB last-level cache (93 -> 81 us; 134 MB in that cache 23 -> 26 us).
+constexpr size_t kMxStream = 256u << 20;
+constexpr int kMxStages = 2;
 template <typename T> constexpr int kMxPer = 16 / (int)sizeof(T);      // columns per thread
 template <typename T> constexpr int kMxRows = 256 * kMxPer<T> / kMxCols;   // rows per workgroup
 template <typename T> inline long mx4_grid(int rows, int K) {
@@ -74,7 +78,7 @@ template <typename T> inline long mx4_grid(int rows, int K) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__ x, int rows, int K, uint8_t* __restrict__ codes,
-                                                           uint8_t* __restrict__ scales, int vec) {
+                                                           uint8_t* __restrict__ scales, int vec, int stream) {
     constexpr int E = kMxPer<T>, LANES = kMxCols / E;                  // threads per row and stage
     const unsigned kbs = (K + kMxCols - 1) / kMxCols, groups = (kbs + kMxStages - 1) / kMxStages;
     const int row = blockIdx.x / groups * kMxRows<T> + threadIdx.x / LANES, t = threadIdx.x % LANES;
@@ -86,7 +90,8 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__
         const int k = (kb0 + u) * kMxCols + t * E, left = K - k;
         const T* at = x + (long)row * K + k;
         if (vec && left >= E) {
-            const Pack16<T> pk = *reinterpret_cast<const Pack16<T>*>(at);
+            const uintx4* from = reinterpret_cast<const uintx4*>(at);
+            const Pack16<T> pk = __builtin_bit_cast(Pack16<T>, stream ? __builtin_nontemporal_load(from) : *from);
 #pragma unroll
             for (int e = 0; e < E; ++e) v[u][e] = to_f32(pk.e[e]);
         } else {
@@ -155,7 +160,10 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint8_t* __re
         for (int e = 0; e < E; ++e) v[e] = mx4_value(c[u] >> (4 * e), b[u]);
         T* to = x + (long)row * K + k;
         if (vec && K - k >= E) {
-            store_chan_vec<T>(to, v);
+            Pack16<T> pk;
+#pragma unroll
+            for (int e = 0; e < E; ++e) pk.e[e] = from_f32<T>(v[e]);
+            __builtin_nontemporal_store(__builtin_bit_cast(uintx4, pk), reinterpret_cast<uintx4*>(to));
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)

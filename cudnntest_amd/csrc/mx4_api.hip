@@ -28,7 +28,8 @@ int check_operand(const char* what, const void* codes, const void* scales) {
 template <typename T> int quantize(int rows, int K, const void* x, void* codes, void* scales, hipStream_t s) {
     const int vec = !misaligned(x, 16) && (size_t)K * sizeof(T) % 16 == 0;
     hipLaunchKernelGGL((mx4_quantize_kernel<T>), dim3(mx4_grid<T>(rows, K)), dim3(256), 0, s,
-                       static_cast<const T*>(x), rows, K, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), vec);
+                       static_cast<const T*>(x), rows, K, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), vec,
+                       (size_t)rows * K * sizeof(T) > kMxStream);
     LAUNCH_CHECK("mx4_quantize");
     return WINO_OK;
 }
