@@ -51,7 +51,7 @@ template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x
     if (p.small) p.logits = place(at, part_bytes(V, T, p.logit.parts));
     if (!backward) {
         if (!p.small) {
-            p.stats = place(at, (size_t)ceil_div(V, p.logit.edge()) * T * sizeof(float2));
+            p.stats = place(at, (size_t)ceil_div(V, p.logit.rows) * T * sizeof(float2));
             p.picked = place(at, (size_t)T * sizeof(float));
         }
     } else {
@@ -161,7 +161,7 @@ template <typename T> struct Call {
         float* picked = reinterpret_cast<float*>(ws + p.picked);
         tile_launch<T, K_INNER, K_INNER>(logits(0, V), CeStats<T>{bias, rows, stats, picked}, p.logit, T_, s);
         LAUNCH_CHECK("ce_stats");
-        hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(T_, 32)), dim3(256), 0, s, stats, picked, rows, T_, ceil_div(V, p.logit.edge()), loss, lse);
+        hipLaunchKernelGGL(ce_join_kernel, dim3(ceil_div(T_, 32)), dim3(256), 0, s, stats, picked, rows, T_, ceil_div(V, p.logit.rows), loss, lse);
         LAUNCH_CHECK("ce_join");
         return WINO_OK;
     }

@@ -201,7 +201,7 @@ inline int tile_grid(int mt, int nt) { return (mt * nt + 7) / 8 * 8; }
 
 // WM x WN waves; a wave owns BM/WM x BN/WN of the tile.  RING stages of LDS, RING - 1 of them in flight.
 template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 || BM * BN * RB * RING > 128 * 128 * 128 * 2 ? 1 : 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
+__global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
     constexpr int WAVES = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
     constexpr bool MX4 = std::is_same<T, mx4_t>::value;
     constexpr int STAGE = RB / 16 * TileElem<T>::piece, STEPS = RB / 32;   // elements of k, multiplies of a lane half
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(256) void tile_join_kernel(const float* __restrict_
 
 // ---- host side -----------------------------------------------------------------------------------
 
-constexpr int kTile = 128;               // edge of a tile
+constexpr int kTile = 128;               // edge of the usual tile
 
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
@@ -568,25 +568,29 @@ inline void tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hip
 template <typename T> constexpr int kStageOf = 8 * TileElem<T>::piece;     // elements of k in 128 bytes
 
 struct TilePick {
-    int big, cols, parts;
-    int deep;                                           // twice the stages in flight, one workgroup to a CU
-    int edge() const { return big ? 256 : kTile; }      // m extent of a tile
+    int rows, cols, parts;      // m and n extent of a tile, parts of the reduction
 };
 
 // The cut with the smallest estimated time.  A CU works through its share of the (tile, part) items; an item takes the
 // longer of its multiplies and its operands' way into LDS; parts are written and read back once in fp32 by one more
 // launch.  `most` bounds the parts (1: the epilogue needs whole sums).  Rates in products / bytes per microsecond and CU,
-// fitted to the measured products of the classifier's sizes.
+// fitted to 24 products in all three kinds of type, each timed with every tile and 1 to 64 parts: the cut it takes is at
+// most 1.2 times the fastest (once 1.33), 1.0 in the middle.  Some of those, us, 256 x 256 / 128 x 128 / 128 x 64 / 64 x 64,
+// whole sums, M x N x K: 16-bit 4096 x 250 x 1000 28 / 15 / 11 / 9, 2048 x 2048 x 2048 52 / 31 / 24 / 29, 2048 x 700 x
+// 32000 in 10 parts 98 (128 x 128: 116 in 4); fp32 10007 x 777 x 1004 250 / 196 / 177 / 155; 4-bit 4096 x 4096 x 4096
+// 43 / 47 / 64 / 72, 500 x 200 x 512 13 / 8 / 6 / 5.
 template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, int cus) {
     constexpr bool F32 = std::is_same<T, float>::value, MX4 = std::is_same<T, mx4_t>::value;
-    const double rate = F32 ? 0.28e6 : MX4 ? 6.5e6 : 2.1e6, rate_big = F32 ? 0.28e6 : MX4 ? 8.0e6 : 2.8e6, bytes = 45e3;
+    const double rate = F32 ? 0.28e6 : MX4 ? 6.5e6 : 2.1e6, bytes = 45e3;
+    // relative to 128 x 128: the large tile draws half the bytes per product, the small ones more
+    const struct { int rows, cols; double factor; } kinds[] = {
+        {256, 256, F32 ? 1.0 : MX4 ? 1.23 : 1.33}, {kTile, kTile, 1.0}, {kTile, 64, F32 ? 0.9 : 0.8}, {kTile, 32, F32 ? 0.8 : 0.5}, {64, 64, F32 ? 0.9 : 0.6}};
     const int stages = ceil_div(K, kStageOf<T>);
-    TilePick best = {0, kTile, 1, 0};
+    TilePick best = {kTile, kTile, 1};
     double least = 1e30;
-    for (int kind = 0; kind < 3; ++kind) {                              // 128 x cols, 256 x 256, 128 x 64 for many rows
-        const int few = N <= 32 && !MX4 ? 32 : N <= 64 ? 64 : kTile;
-        if ((kind == 1 && (M <= kTile || N <= kTile)) || (kind == 2 && (!F32 || few < kTile))) continue;
-        const int cols = kind == 1 ? 256 : kind == 2 ? 64 : few, rows = kind == 1 ? 256 : kTile;
+    for (const auto& kind : kinds) {
+        const int rows = kind.rows, cols = kind.cols;
+        if ((rows == 256 && (M <= kTile || N <= kTile)) || (cols == 32 && (MX4 || N > 64))) continue;
         const long tiles = (long)ceil_div(M, rows) * ceil_div(N, cols);
         for (int parts = 1; parts <= most && parts <= std::max(1, stages / 2); parts += parts < 8 ? 1 : parts / 4) {
             const int split = ceil_div(stages, parts);
@@ -594,14 +598,14 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
             const long items = tiles * parts;
             if (parts > 1 && (items > 4L * cus || (size_t)parts * M * N * 4 > (64u << 20))) break;
             const double k = (double)split * kStageOf<T>;
-            const double mul = (double)rows * cols * k / (kind == 1 ? rate_big : kind == 2 ? 0.88 * rate : rate);
+            const double mul = (double)rows * cols * k / (rate * kind.factor);
             const double move = (double)(rows + cols) * split * 128 / bytes;
             // one small tile alone on its CU waits for its own loads
-            const double item = std::max(mul, move) * (kind != 1 && items <= cus ? 1.25 : 1.0);
+            const double item = std::max(mul, move) * (rows < 256 && items <= cus ? 1.25 : 1.0);
             const double t = ceil_div(items, cus) * item + (parts > 1 ? 4.0 + (double)parts * M * N * 8 / 4e6 : 0.0);
             if (t < least) {
                 least = t;
-                best = {kind == 1, cols, parts, !kind && cols == kTile && items <= cus};
+                best = {rows, cols, parts};
             }
         }
     }
@@ -612,15 +616,12 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
 template <typename T, int AO, int BO, class Epi>
 inline void tile_launch(const TileArgs& g, const Epi& epi, const TilePick& pick, int cover, hipStream_t s) {
     constexpr int RB = std::is_same<T, mx4_t>::value ? 64 : 128;
-    if (pick.big) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
+    if (pick.rows == 256) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
+    if (pick.rows == 64) return tile_launch_as<T, AO, BO, 64, 64, 2, 2, RB, RB == 64 ? 5 : 3>(g, epi, pick.parts, cover, s);
     if constexpr (RB == 128)            // (a 4-bit stage of 32 rows is less than a load per wave)
         if (pick.cols == 32) return tile_launch_as<T, AO, BO, kTile, 32, 4, 1, RB, 4>(g, epi, pick.parts, cover, s);
-    switch (pick.cols) {
-    case 64: return tile_launch_as<T, AO, BO, kTile, 64, 4, 1, RB, RB == 64 ? 5 : 3>(g, epi, pick.parts, cover, s);
-    default:
-        if (pick.deep) return tile_launch_as<T, AO, BO, kTile, kTile, 2, 2, RB, RB == 64 ? 8 : 4>(g, epi, pick.parts, cover, s);
-        return tile_launch_as<T, AO, BO, kTile, kTile, 2, 2, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
-    }
+    if (pick.cols == 64) return tile_launch_as<T, AO, BO, kTile, 64, 4, 1, RB, RB == 64 ? 5 : 3>(g, epi, pick.parts, cover, s);
+    return tile_launch_as<T, AO, BO, kTile, kTile, 2, 2, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
 }
 
 inline size_t part_bytes(int M, int N, int parts) { return (size_t)parts * N * round_up(M, 4) * sizeof(float); }
