@@ -9,11 +9,17 @@
 // 64 of its logits in registers, so the softmax statistics of a tile need no exchange between lanes but one.
 // Forward: every tile leaves (max, sum of exp) per row, 8 bytes for 128 logits, and one kernel joins them.  Backward:
 // the vocabulary is taken in pieces; a piece's dl (in the tensors' type) goes to scratch and feeds the two products.
+// Rounding dl to 16 bits adds about as much error as rounding the gradients themselves.  Over many rows these average;
+// up to kTwinRows rows a gradient can hang on a few entries of dl, so dl is then kept as two 16-bit values, what the type
+// holds and what it leaves over, and the two products run over both (their reduction twice as long, in calls that are
+// bound by their weights' bytes).
 #pragma once
 #include "common.hpp"
 #include "tile_gemm.hpp"
 
 namespace wino {
+
+constexpr int kTwinRows = 256;
 
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -126,6 +132,12 @@ template <typename T> __device__ __forceinline__ float dl_of(float l, const ExpF
     return ignored ? 0.f : (p(l) - (hit ? 1.f : 0.f)) * weight;
 }
 
+// what rounding to T leaves of a value (0 where there is nothing finite to leave)
+template <typename T> __device__ __forceinline__ float left_over(float v) {
+    const float d = v - to_f32(from_f32<T>(v));
+    return d - d == 0.f ? d : 0.f;
+}
+
 // dl[t][v - v0] of a piece of the vocabulary, zeros around it (rows up to row_end, columns up to pitch)
 template <typename T> struct CeDl {
     const T* bias;          // of the piece
@@ -135,8 +147,9 @@ template <typename T> struct CeDl {
     const float* scale;     // one factor in device memory, or null
     int v0;                 // first class of the piece
     T* dl;
-    long pitch;             // elements, a multiple of 8
-    int row_end;
+    long pitch;             // elements from row to row
+    int width;              // of a row, a multiple of 8; twin: followed by `width` elements of what rounding left over
+    int row_end, twin;
     template <int BM, int BN, int WM, int WN, int MI, int NI>
     __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char* lds) const {
         const float f = scale ? *scale : 1.f;
@@ -157,7 +170,7 @@ template <typename T> struct CeDl {
             const int first = m0 + wm * MI * 32;
             none[n] = !__any(hit[n] >= first && hit[n] < first + MI * 32);
         }
-        tile_store<T, WM, WN, MI, NI>(dl, pitch, m0, n0, row_end, (int)pitch, wm, wn, l32, lh, lds, false, [&](int i, int q, int n, float (&v)[4]) {
+        auto value = [&](int i, int q, int n, float (&v)[4]) {
             const int m = m0 + (wm * MI + i) * 32 + 8 * q + 4 * lh;
             const ExpFrom<T> p(z[n]);
             if (plain && none[n]) {
@@ -170,7 +183,14 @@ template <typename T> struct CeDl {
                 const float b = bias && m + e < g.M ? to_f32(bias[m + e]) : 0.f;
                 v[e] = m + e < g.M ? dl_of(acc[i][n][4 * q + e] + b, p, hit[n] == m + e, weight[n], ignored[n]) : 0.f;
             }
-        });
+        };
+        tile_store<T, WM, WN, MI, NI>(dl, pitch, m0, n0, row_end, width, wm, wn, l32, lh, lds, false, value);
+        if (twin)
+            tile_store<T, WM, WN, MI, NI>(dl + width, pitch, m0, n0, row_end, width, wm, wn, l32, lh, lds, false, [&](int i, int q, int n, float (&v)[4]) {
+                value(i, q, n, v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = left_over<T>(v[e]);
+            });
     }
 };
 
@@ -265,7 +285,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(CeParts<T> p, CeRows rows
 template <typename T>
 __global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int T_rows) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    const int quads = (int)(o.pitch / 4);
+    const int quads = o.width / 4;
     const int t = (int)(i / quads), m = (int)(i - (long)t * quads) * 4;
     if (t >= o.row_end) return;
     const bool in = t < T_rows;
@@ -282,12 +302,17 @@ __global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int
         v[e] = in && m + e < o.rows.V ? dl_of(l[e] + b, ExpFrom<T>(z), target == m + e, weight, ignored) : 0.f;
     }
     store4<T>(o.dl + (long)t * o.pitch + m, v, 4, true);
+    if (o.twin) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = left_over<T>(v[e]);
+        store4<T>(o.dl + (long)t * o.pitch + o.width + m, v, 4, true);
+    }
 }
 
 // dbias[v] = scale * sum_t dl[t][v], fp32, rows in a fixed order: 64 classes x 16 groups of rows per workgroup
 template <typename T>
-__global__ __launch_bounds__(1024) void ce_bias_kernel(const T* __restrict__ dl, long pitch, int rows, int V, const float* __restrict__ scale,
-                                                       T* __restrict__ dbias) {
+__global__ __launch_bounds__(1024) void ce_bias_kernel(const T* __restrict__ dl, long pitch, int width, int twin, int rows, int V,
+                                                       const float* __restrict__ scale, T* __restrict__ dbias) {
     __shared__ float ex[16][64];
     const int c = threadIdx.x & 63, part = threadIdx.x >> 6;
     const int v = blockIdx.x * 64 + c;
@@ -302,6 +327,8 @@ __global__ __launch_bounds__(1024) void ce_bias_kernel(const T* __restrict__ dl,
             for (int u = 0; u < 8; ++u) s += a[u];
         }
         for (; t < rows; t += 16) s += to_f32(dl[(long)t * pitch + v]);
+        if (twin)
+            for (t = part; t < rows; t += 16) s += to_f32(dl[(long)t * pitch + width + v]);
     }
     ex[part][c] = s;
     __syncthreads();
@@ -311,10 +338,11 @@ __global__ __launch_bounds__(1024) void ce_bias_kernel(const T* __restrict__ dl,
     dbias[v] = from_f32<T>(s * (scale ? *scale : 1.f));
 }
 
-// f16 has five exponent bits: dl is stored times 2^(15 - e) with 2^e just above the largest weight, and the products
-// are multiplied back.  |exp(l - lse) - hit| <= 1, so nothing overflows (2^15 < 65504), and values down to 2^-39 of
-// the largest weight are kept.  out[0] = the factor, out[1] = its inverse; powers of two, so both are exact.
-__global__ __launch_bounds__(1024) static void ce_scale_kernel(const float* __restrict__ grad, CeRows rows, int T, float* __restrict__ out) {
+// 16-bit dl is stored relative to the largest weight: with equal weights (a mean over the rows) the targets' entries are
+// then close to -1, which the type holds well, instead of all sharing the rounding error of the weight.  f16 in addition
+// has only five exponent bits: times 2^15 (|exp(l - lse) - hit| <= 1, so nothing overflows), which keeps values down to
+// 2^-39 of the largest weight.  out[0] = the factor, out[1] = its inverse, applied to the fp32 sums.
+__global__ __launch_bounds__(1024) static void ce_scale_kernel(const float* __restrict__ grad, CeRows rows, int T, float top, float* __restrict__ out) {
     __shared__ float ex[1024];
     float mx = 0.f;
     for (int t = threadIdx.x; t < T; t += 1024)
@@ -326,13 +354,10 @@ __global__ __launch_bounds__(1024) static void ce_scale_kernel(const float* __re
         __syncthreads();
     }
     if (threadIdx.x != 0) return;
-    int e = 15;                                                        // no weight at all, or none that is finite: 1
-    if (ex[0] > 0.f && ex[0] <= 3.4028235e38f) {
-        frexpf(ex[0], &e);
-        e = max(e, -100);
-    }
-    out[0] = ldexpf(1.f, 15 - e);
-    out[1] = ldexpf(1.f, e - 15);
+    // no weight at all, or none that is finite: 1
+    const float g = ex[0] > 0.f && ex[0] <= 3.4028235e38f ? fmaxf(ex[0], 1e-30f) : top;
+    out[0] = top / g;
+    out[1] = g / top;
 }
 
 // rows of `cols` elements copied to a 16-byte aligned pitch, zeros behind them

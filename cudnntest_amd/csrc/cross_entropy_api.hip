@@ -10,7 +10,7 @@ bool valid_dtype(int d) { return d == WINO_F32 || d == WINO_F16 || d == WINO_BF1
 bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
 constexpr int kMaxCols = 1 << 21;                     // the kernels' 32-bit offsets inside a tile rest on it
-constexpr long kMaxTiles = 1L << 30;
+constexpr long kMaxTiles = 1L << 27;                  // of 128 x 128
 constexpr size_t kPieceBytes = 128u << 20;            // dl of one piece of the vocabulary: half of the last-level cache
 
 // Where everything is in the workspace, and how the problem is cut.  The same function sizes the workspace and drives
@@ -22,6 +22,7 @@ struct Plan {
     TilePick logit, dx_cut, dw_cut;     // how the three products are cut
     int rows;                           // of dl: T rounded up to a stage
     int piece;                          // classes per piece (backward)
+    bool twin;                          // dl as two 16-bit values
     size_t x, w, logits, stats, picked, scale, dl, dx, dw, total;
 };
 
@@ -44,11 +45,15 @@ template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x
     p.pitch_x = p.pad_x ? padded : D;
     p.pitch_w = p.pad_w ? padded : D;
     p.logit = tile_pick<E>(V, T, D, kMostParts, cus);
-    p.small = p.logit.parts > 1;
+    p.rows = (int)round_up(T, 64);
+    p.twin = e == 2 && T <= kTwinRows;
+    const int two = p.twin ? 2 : 1;
+    p.small = p.logit.parts > 1 && (!backward || (size_t)p.rows * round_up(V, 128) * e * two <= kPieceBytes);
     size_t at = 0;
     if (p.pad_x) p.x = place(at, (size_t)T * p.pitch_x * e);
     if (p.pad_w) p.w = place(at, (size_t)V * p.pitch_w * e);
     if (p.small) p.logits = place(at, part_bytes(V, T, p.logit.parts));
+    else p.logit = tile_pick<E>(V, T, D, 1, cus);
     if (!backward) {
         if (!p.small) {
             p.stats = place(at, (size_t)ceil_div(V, p.logit.rows) * T * sizeof(float2));
@@ -56,13 +61,12 @@ template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x
         }
     } else {
         p.scale = place(at, 2 * sizeof(float));
-        p.rows = (int)round_up(T, 64);
-        const size_t fit = kPieceBytes / ((size_t)p.rows * e) / 256 * 256;
+        const size_t fit = kPieceBytes / ((size_t)p.rows * e * two) / 256 * 256;
         p.piece = p.small ? V : (int)std::min<size_t>(V, std::max<size_t>(fit, 256));
-        p.dl = place(at, (size_t)p.rows * round_up(p.piece, 128) * e);
+        p.dl = place(at, (size_t)p.rows * round_up(p.piece, 128) * e * two);
         if (!p.small) p.logit = tile_pick<E>(p.piece, T, D, 1, cus);
-        p.dx_cut = tile_pick<E>(D, T, p.piece, kMostParts, cus);
-        p.dw_cut = tile_pick<E>(D, p.piece, T, kMostParts, cus);
+        p.dx_cut = tile_pick<E>(D, T, p.piece * two, kMostParts, cus);
+        p.dw_cut = tile_pick<E>(D, p.piece, T * two, kMostParts, cus);
         if (p.dx_cut.parts > 1 || p.piece < V) p.dx = place(at, part_bytes(D, T, p.dx_cut.parts));
         if (p.dw_cut.parts > 1) p.dw = place(at, part_bytes(D, p.piece, p.dw_cut.parts));
     }
@@ -100,7 +104,7 @@ template <typename T> TileOperand outer(const T* p, long pitch, int k_rows) {
 
 template <typename T> int pad_rows(const T* x, long rows, int cols, T* y, int pitch, hipStream_t s) {
     const long n = rows * (pitch / 4);
-    if (ceil_div(n, 256) <= 0 || n / 256 > 0x7ffffff0L) return fail(WINO_ERR_UNSUPPORTED, "pad_rows: %ld rows of %d", rows, cols);
+    if (n / 256 > 0x7ffffff0L) return fail(WINO_ERR_UNSUPPORTED, "pad_rows: %ld rows of %d", rows, cols);
     hipLaunchKernelGGL((pad_rows_kernel<T>), dim3(ceil_div(n, 256)), dim3(256), 0, s, x, rows, cols, y, pitch);
     LAUNCH_CHECK("pad_rows");
     return WINO_OK;
@@ -170,9 +174,9 @@ template <typename T> struct Call {
         int rc = operands();
         if (rc) return rc;
         float* scale = nullptr;
-        if (std::is_same<T, f16_t>::value) {
+        if (sizeof(T) == 2) {
             scale = reinterpret_cast<float*>(ws + p.scale);
-            hipLaunchKernelGGL(ce_scale_kernel, dim3(1), dim3(1024), 0, s, grad, rows, T_, scale);
+            hipLaunchKernelGGL(ce_scale_kernel, dim3(1), dim3(1024), 0, s, grad, rows, T_, std::is_same<T, f16_t>::value ? 32768.f : 1.f, scale);
             LAUNCH_CHECK("ce_scale");
         }
         const float* back = scale ? scale + 1 : nullptr;
@@ -184,12 +188,13 @@ template <typename T> struct Call {
         const TileStore<T> dx_store = {dx, D, nullptr, back, 0};
         for (int v0 = 0; v0 < V; v0 += p.piece) {
             const int n = std::min(p.piece, V - v0);
-            const long pitch = round_up(n, 128);
-            const CeDl<T> out = {bias ? bias + v0 : nullptr, rows, lse, grad, scale, v0, dl, pitch, p.rows};
+            const int width = (int)round_up(n, 128);
+            const long pitch = p.twin ? 2L * width : width;
+            const CeDl<T> out = {bias ? bias + v0 : nullptr, rows, lse, grad, scale, v0, dl, pitch, width, p.rows, p.twin};
             if (p.small) {
                 CeParts<T> parts;
                 if ((rc = partial_logits(&parts))) return rc;
-                hipLaunchKernelGGL((ce_dl_kernel<T>), dim3(ceil_div((long)p.rows * (pitch / 4), 256)), dim3(256), 0, s, parts, out, T_);
+                hipLaunchKernelGGL((ce_dl_kernel<T>), dim3(ceil_div((long)p.rows * (width / 4), 256)), dim3(256), 0, s, parts, out, T_);
             } else {
                 tile_launch<T, K_INNER, K_INNER>(logits(v0, n), out, p.logit, p.rows, s);
             }
@@ -201,6 +206,12 @@ template <typename T> struct Call {
                 g.M = D;
                 g.N = T_;
                 g.K = n;
+                if (p.twin) {           // over dl, then over what it leaves; w from its start again
+                    g.K = (int)round_up(n, kStageOf<T>);
+                    g.passes = 2;
+                    g.a_turn = -(long)g.K * g.a.pitch;
+                    g.b_turn = (width - g.K) * (long)sizeof(T);
+                }
                 if (dx_direct) tile_launch<T, K_OUTER, K_INNER>(g, dx_store, p.dx_cut, T_, s);
                 else tile_launch<T, K_OUTER, K_INNER>(g, TilePart{dx_part, d4, v0 > 0}, p.dx_cut, T_, s);
                 LAUNCH_CHECK("ce_dx");
@@ -212,6 +223,12 @@ template <typename T> struct Call {
                 g.M = D;
                 g.N = n;
                 g.K = T_;
+                if (p.twin) {
+                    g.K = p.rows;
+                    g.passes = 2;
+                    g.a_turn = -(long)g.K * g.a.pitch;
+                    g.b_turn = -(long)g.K * g.b.pitch + width * (long)sizeof(T);
+                }
                 const TileStore<T> store = {dw + (long)v0 * D, D, nullptr, back, 0};
                 if (p.dw_cut.parts == 1) {
                     tile_launch<T, K_OUTER, K_OUTER>(g, store, p.dw_cut, n, s);
@@ -224,7 +241,7 @@ template <typename T> struct Call {
                 LAUNCH_CHECK("ce_dw");
             }
             if (dbias) {
-                hipLaunchKernelGGL((ce_bias_kernel<T>), dim3(ceil_div(n, 64)), dim3(1024), 0, s, dl, pitch, T_, n, back, dbias + v0);
+                hipLaunchKernelGGL((ce_bias_kernel<T>), dim3(ceil_div(n, 64)), dim3(1024), 0, s, dl, pitch, width, p.twin, T_, n, back, dbias + v0);
                 LAUNCH_CHECK("ce_bias");
             }
         }

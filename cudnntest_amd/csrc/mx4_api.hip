@@ -11,12 +11,12 @@ bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p
 
 // limits that the kernels' 32-bit offsets inside a tile rest on
 constexpr int kMaxCols = 1 << 21;
-constexpr long kMaxTiles = 1L << 30;
+constexpr long kMaxTiles = 1L << 27;            // of 128 x 128
 
 int check_shape(const char* what, long rows, int K) {
     if (rows <= 0 || K <= 0) return fail(WINO_ERR_INVALID, "%s: sizes must be positive (rows %ld, K %d)", what, rows, K);
     if (K > kMaxCols) return fail(WINO_ERR_UNSUPPORTED, "%s: K = %d, at most %d", what, K, kMaxCols);
-    if (mx4_grid<float>(rows, K) > kMaxTiles) return fail(WINO_ERR_UNSUPPORTED, "%s: %ld rows of %d", what, rows, K);
+    if (mx4_grid<float>(rows, K) > 0x7fffffffL) return fail(WINO_ERR_UNSUPPORTED, "%s: %ld rows of %d", what, rows, K);
     return WINO_OK;
 }
 int check_operand(const char* what, const void* codes, const void* scales) {

@@ -53,9 +53,12 @@ struct TileOperand {
 
 struct TileArgs {
     TileOperand a, b;
-    int M, N, K;            // K in elements
+    int M, N, K;            // K in elements (of one pass)
+    int passes;             // 2: the reduction runs twice, the operands starting over at a_turn / b_turn (0 counts as 1)
+    long a_turn, b_turn;    // bytes added behind a pass's last stage
     int mt, nt;             // tiles along m and n
     int stages, split;      // stages in all, stages per part of the reduction (grid.y parts)
+    int pass, tail_at;      // stages of a pass; the one of them that does not exist in full, or -1 (set by the launch)
 };
 
 // the j-th of a lane's four scale bytes: a compile-time operand of the instruction
@@ -154,11 +157,12 @@ template <typename T, int ORDER, int EXT, int WAVES, int RB> struct TileSide {
         for (int q = kLoads * P / OF; q < kLoads * (P + 1) / OF; ++q) dma_piece(base, off[q], dst + (wave * kLoads + q) * 1024);
         if (P == OF - 1) base += (uint64_t)op.step;
     }
-    // the last stage of a reduction that does not fill it
+    // a stage that does not exist in full
     __device__ __forceinline__ void load_tail(const TileOperand& op, int org, int k_left, unsigned dst, int wave, int lane) {
 #pragma unroll
         for (int q = 0; q < kLoads; ++q)
             dma_piece(base, source(op, org, q, wave, lane, k_left), dst + (wave * kLoads + q) * 1024);
+        base += (uint64_t)op.step;
     }
     // piece j of block `blk` (32 rows or columns) for this lane
     __device__ __forceinline__ uintx4 fragment(const char* st, int blk, int j, int lane) const {
@@ -211,6 +215,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     constexpr int SROW = RB / 16, SCA = (BM * SROW + 1023) / 1024, SCB = (BN * SROW + 1023) / 1024;
     constexpr int SC = MX4 ? (SCA + SCB) * 1024 : 0;
     constexpr int SLOT = SA::kBytes + SB::kBytes + SC;
+    constexpr bool TWO = AO == K_OUTER && sizeof(T) == 2;              // the products that run in two passes
     __shared__ __align__(1024) char lds[RING * SLOT];
 
     int tm, tn;
@@ -221,12 +226,15 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     const int wm = wave / WN, wn = wave % WN;
     const int l32 = lane & 31, lh = lane >> 5;
     const int first = blockIdx.y * g.split, last = min(first + g.split, g.stages);
-    const bool ragged = last == g.stages && g.K % STAGE != 0;   // the last stage is a part of one
 
     SA sa;
     SB sb;
     sa.init(g.a, m0, first, wave, lane);
     sb.init(g.b, n0, first, wave, lane);
+    if (TWO && first >= g.pass) {
+        sa.base += (uint64_t)g.a_turn;
+        sb.base += (uint64_t)g.b_turn;
+    }
     const unsigned lds0 = lds_addr(lds);
     // mx4: scale bytes as 16-byte pieces (16 / SROW rows), one load each by the first waves
     uint64_t sc_base = 0;
@@ -257,13 +265,17 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
 
     auto issue = [&](int s, int slot) {
         const unsigned dst = lds0 + slot * SLOT;
-        if (ragged && s == last - 1) {
-            const int k0 = s * STAGE;
-            sa.load_tail(g.a, m0, SA::left(g.a, g.K, k0), dst, wave, lane);
-            sb.load_tail(g.b, n0, SB::left(g.b, g.K, k0), dst + SA::kBytes, wave, lane);
+        const int local = TWO && s >= g.pass ? s - g.pass : s;
+        if (local == g.tail_at) {
+            sa.load_tail(g.a, m0, SA::left(g.a, g.K, local * STAGE), dst, wave, lane);
+            sb.load_tail(g.b, n0, SB::left(g.b, g.K, local * STAGE), dst + SA::kBytes, wave, lane);
         } else {
             sa.load(g.a, dst, wave);
             sb.load(g.b, dst + SA::kBytes, wave);
+        }
+        if (TWO && local == g.pass - 1) {
+            sa.base += (uint64_t)g.a_turn;
+            sb.base += (uint64_t)g.b_turn;
         }
         if constexpr (MX4) {
             if (wave < SCA + SCB) {
@@ -299,10 +311,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     auto multiply = [&](int s, auto jc, auto tail) {
         constexpr int J = decltype(jc)::value;
         if constexpr (decltype(tail)::value && !MX4) {
-            // pieces past the end of the reduction: zero wherever k is inner (they were read from elsewhere in the
+            // pieces past the end of the reduction (two passes: whole stages): zero wherever k is inner (they were read from elsewhere in the
             // row).  A k-outer operand needs no mask beside a k-inner one; where both are k-outer, the rows past
             // the end exist and one of the two holds zeros in them.
-            const bool in = STEPS * lh + J < (g.K - s * STAGE + TileElem<T>::piece - 1) / TileElem<T>::piece;
+            const bool in = (TWO && g.passes > 1) || STEPS * lh + J < (g.K - s * STAGE + TileElem<T>::piece - 1) / TileElem<T>::piece;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
                 if (AO == K_INNER && !in) fa[J & 1][i] = uintx4{0, 0, 0, 0};
@@ -321,6 +333,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     // in the first two and B's in the last two (16-bit 8192 x 4096 x 16384: 943 -> 902 us), with two all of them at once
     // (4-bit: a split there gains nothing).
     constexpr bool SPREAD = STEPS == 4;
+    auto plain_stage = [&](int s) {                                    // (the others go in one piece)
+        const int local = TWO && s >= g.pass ? s - g.pass : s;
+        return local != g.tail_at && (!TWO || local != g.pass - 1);
+    };
     bool pending = false;
     int refill = 0;
     auto share = [&](auto pc) {
@@ -367,7 +383,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
         read(slot, j0);
         read_scales(slot, 1);
         __builtin_amdgcn_sched_barrier(0);
-        pending = SPREAD && !MX4 && s + RING < (ragged ? last - 1 : last);      // (a partial stage goes in one piece)
+        pending = SPREAD && !MX4 && s + RING < last && plain_stage(s + RING);
         if (pending) share(j0);
         else if (s + RING < last) issue(s + RING, refill);
         __builtin_amdgcn_sched_barrier(0);
@@ -382,6 +398,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     }
     all_but_last(last - 1, slot, std::true_type{});
     multiply(last - 1, j_last, std::true_type{});
+    asm volatile("" ::: "memory");                                    // (the last reads stay above the epilogue's barrier)
     wait_loads<0>();
     epi.template run<BM, BN, WM, WN, MI, NI>(acc, g, m0, n0, wm, wn, l32, lh, lds);
 }
@@ -558,7 +575,11 @@ inline void tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hip
     const bool mx4 = std::is_same<T, mx4_t>::value;
     g.a.step = mx4 ? g.a.rows * (long)RB : AO == K_INNER ? RB : g.a.pitch * stage;
     g.b.step = mx4 ? g.b.rows * (long)RB : BO == K_INNER ? RB : g.b.pitch * stage;
-    g.stages = ceil_div(g.K, stage);
+    g.passes = std::max(g.passes, 1);
+    g.pass = ceil_div(g.K, stage);
+    // with two passes K is a whole number of stages, of which a k-outer A may hold a little less
+    g.tail_at = g.passes > 1 ? (AO == K_OUTER && g.a.rows < g.K ? g.pass - 1 : -1) : g.K % stage ? g.pass - 1 : -1;
+    g.stages = g.passes * g.pass;
     g.split = ceil_div(g.stages, parts);
     parts = ceil_div(g.stages, g.split);
     hipLaunchKernelGGL((tile_gemm_kernel<T, AO, BO, BM, BN, WM, WN, RB, RING, Epi>), dim3(tile_grid(g.mt, g.nt), parts), dim3(64 * WM * WN), 0, s, g, epi);

@@ -362,9 +362,9 @@ int wino_linear_cross_entropy(int dtype, int T, int D, int V, const void *x, con
 /* Gradients of sum_t grad[t] * loss[t], lse from the call above: with dl[t][v] = grad[t] (exp(l[t][v] - lse[t]) -
  * [v == target[t]]) (zeros for an ignored row, NaN for a row with an invalid target)
  *     dx = dl w,   dw = dl^T x,   dbias[v] = sum_t dl[t][v]
- * in `dtype`; any of the three may be NULL.  The logits are computed again, a piece of the vocabulary at a time; dl is rounded
- * to `dtype` before the products (in f16 scaled by a power of two taken from the largest weight, so that small probabilities
- * do not underflow), sums are fp32. */
+ * in `dtype`; any of the three may be NULL.  The logits are computed again, a piece of the vocabulary at a time; dl
+ * enters the products in `dtype`, relative to the largest weight (for 256 rows and fewer as two such values, so that no
+ * rounding of dl shows in the gradients); sums are fp32. */
 int wino_linear_cross_entropy_backward(int dtype, int T, int D, int V, const void *x, const void *w, const void *bias,
                                        const long long *target, long long ignore_index, const float *grad, const float *lse,
                                        void *dx, void *dw, void *dbias, void *workspace, size_t workspace_bytes, void *stream);

@@ -108,7 +108,8 @@ class Ce:
         dp = p * (fin + (self.lse_tol + E32 * self.lse.abs()).unsqueeze(1) + (4 * spread + 8) * E32) + 2.0 ** -126
         gmax = g.abs().max()
         floor = gmax * 2.0 ** -39 if dt == torch.float16 else TINY[dt]
-        dd = (dp + 2 * E32 * (p + hot)) * g.abs().unsqueeze(1) + d.abs() * U[dt] + floor
+        # (six more roundings: the subtraction, the row's weight made relative to the largest, its product, the way back)
+        dd = (dp + 6 * E32 * (p + hot)) * g.abs().unsqueeze(1) + d.abs() * U[dt] + floor
         dd = torch.where(keep.unsqueeze(1), dd, torch.zeros_like(dd))
         ad = d.abs() + dd
         self.dx, self.dw, self.db = d @ W, d.t().contiguous() @ X, d.sum(0)

@@ -210,3 +210,83 @@ def test_in_a_graph(T, V, dtype):
         torch.cuda.synchronize()
         for a, c in zip(out, step()):
             assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,D,V", [(256, 40, 700), (257, 40, 700), (255, 72, 33), (193, 64, 40000), (64, 200, 129), (200, 16, 140000)])
+def test_dl_in_two_values(T, D, V, dtype):
+    """Up to 256 rows dl is kept as two 16-bit values: the gradients' error is that of their own rounding, nothing of dl's."""
+    x, w, target, b, grad = problem(T, D, V, dtype)
+    loss, lse, dx, dw, db = check(x, w, target, b, grad)
+    if T > 256:
+        return
+    ref = Ce(x, w, target, b, -100, grad)
+    for got, want in ((dx, ref.dx), (dw, ref.dw), (db, ref.db)):
+        best = (want.to(dtype).double() - want).norm()     # rounded once
+        assert (got.double() - want).norm() <= 1.05 * best + 2e-5 * want.norm()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_equal_weights_share_no_rounding(dtype):
+    """A mean over 1000 rows: 1/1000 is no 16-bit number, and its rounding must not scale the whole gradient."""
+    x, w, target, b, grad = problem(1000, 64, 5000, dtype, std=0.1)
+    grad.fill_(1.0 / 1000)
+    ref = Ce(x, w, target, b, -100, grad)
+    _, lse = ops.linear_cross_entropy(x, w, target, bias=b)
+    dx, dw, db = ops.linear_cross_entropy_backward(grad, x, w, target, lse, bias=b)
+    for got, want in ((dx, ref.dx), (dw, ref.dw)):
+        # the projection on the exact gradient: a common factor would show as up to 2^-9 (bf16), 2^-12 (f16)
+        factor = (got.double() * want).sum() / (want * want).sum()
+        assert abs(factor.item() - 1.0) < 2.0 ** -11
+
+
+def test_weights_past_four_gigabytes():
+    """w of 4.6 GB: the rows' statistics and the gradients of the last classes."""
+    T, D, V = 48, 16384, 140_000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.empty(V, D, dtype=torch.bfloat16, device="cuda")
+    for v in range(0, V, 10000):
+        w[v:v + 10000] = torch.randn(10000, D, generator=g, device="cuda") / 128
+    x = torch.randn(T, D, generator=g, device="cuda").to(torch.bfloat16)
+    target = torch.randint(V - 2000, V, (T,), generator=g, device="cuda")
+    grad = torch.full((T,), 1.0, device="cuda")
+    loss, lse = ops.linear_cross_entropy(x, w, target)
+    l = torch.cat([x.double() @ w[v:v + 10000].double().t().contiguous() for v in range(0, V, 10000)], 1)
+    want = torch.logsumexp(l, 1)
+    assert (lse - want).abs().max() < 1e-4
+    assert (loss - (want - l[torch.arange(T), target])).abs().max() < 1e-4
+    dx, dw, _ = ops.linear_cross_entropy_backward(grad, x, w, target, lse)
+    d = (l - want[:, None]).exp()
+    d[torch.arange(T, device="cuda"), target] -= 1.0
+    ref = d[:, -2000:].t().contiguous() @ x.double()
+    assert (dw[-2000:].double() - ref).norm() / ref.norm() < 2.5e-3
+    ref = sum(d[:, v:v + 10000] @ w[v:v + 10000].double() for v in range(0, V, 10000))
+    assert (dx.double() - ref).norm() / ref.norm() < 2.5e-3
+
+
+def test_two_streams_and_threads_at_once():
+    import threading
+    jobs = [problem(70 + k, 256, 900, torch.bfloat16, seed=k) for k in range(2)]
+
+    def step(p):
+        x, w, target, b, grad = p
+        loss, lse = ops.linear_cross_entropy(x, w, target, bias=b)
+        return (loss,) + ops.linear_cross_entropy_backward(grad, x, w, target, lse, bias=b)
+    want = [step(p) for p in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(8):
+                got[k].append(step(jobs[k]))
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(got[k]) == 8
+        for out in got[k]:
+            assert all(torch.equal(a, c) for a, c in zip(out, want[k]))

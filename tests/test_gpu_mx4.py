@@ -168,3 +168,44 @@ def test_linear_in_a_graph_and_on_another_stream(M, N, K):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, ops.mx4_linear(x, w))
+
+
+def test_codes_past_four_gigabytes():
+    """Weights whose codes pass 2^32 bytes: the last rows' results are those of these rows on their own, bit for bit."""
+    N, K = 270_000, 32768
+    wq = ops.Mx4._empty(N, K, torch.device("cuda", 0))
+    assert wq.codes.numel() > 1 << 32
+    part = features(1000, K, torch.float16, 1).cuda()
+    big = torch.empty(N, K, dtype=torch.float16, device="cuda")
+    for r in range(0, N, 1000):
+        torch.mul(part, 1.0 + (r % 7000) / 10000.0, out=big[r:r + 1000])
+    ops.mx4_quantize(big, out=wq)
+    tail = ops.mx4_quantize(big[-300:].clone())
+    kb = K // 128
+    assert torch.equal(wq.codes.view(kb, N, 64)[:, -300:], tail.codes.view(kb, 300, 64))
+    del big
+    for M in (1, 5, 20, 200):
+        x = features(M, K, torch.float16, 2).cuda()
+        y, want = ops.mx4_linear(x, wq), ops.mx4_linear(x, tail)
+        if M <= 16:                                        # one kernel, one order of the sum
+            assert torch.equal(y[:, -300:], want)
+        else:
+            assert (y[:, -300:].float() - want.float()).abs().max() <= 2 * 2.0 ** -11 * want.float().abs().max()
+    back = ops.mx4_dequantize(wq, torch.float16)
+    assert torch.equal(back[-300:], ops.mx4_dequantize(tail, torch.float16))
+
+
+def test_two_streams_at_once():
+    """Calls on two streams overlap: each has its own workspace and output."""
+    jobs = [(features(M, 4096, torch.bfloat16, M).cuda(), ops.mx4_quantize(features(1000, 4096, torch.bfloat16, M + 1).cuda())) for M in (200, 203)]
+    want = [ops.mx4_linear(x, w) for x, w in jobs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k, (x, w) in enumerate(jobs):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(ops.mx4_linear(x, w))
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(y, want[k]) for y in got[k])
