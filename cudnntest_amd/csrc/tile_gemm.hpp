@@ -204,6 +204,15 @@ __device__ __forceinline__ bool tile_of(int id, int mt, int nt, int& tm, int& tn
 inline int tile_grid(int mt, int nt) { return (mt * nt + 7) / 8 * 8; }
 
 // WM x WN waves; a wave owns BM/WM x BN/WN of the tile.  RING stages of LDS, RING - 1 of them in flight.
+//
+// What bounds it (256 x 256, bf16 of random values, 8192 x 4096 outputs): K = 8192 takes 419 us, 1.31 PFLOP/s, K = 2048 in
+// two rounds 126 us: 14 us of a round are its first loads and its stores.  Without the loads the first takes about a
+// seventh less, without the LDS reads as well, without the multiplies (loads and LDS reads alone) 165 of 265 us at
+// K = 4096: the CU's request path (64 KB of operands per 2048 clocks of multiplies), LDS and the matrix pipe are each
+// busy for more than half of the time, and on zeros instead of random values the same launch runs a quarter faster (the
+// clock follows the data).  4-bit 4096 x 8192 x 8192: 155 us, 3.5 PFLOP/s, the same bytes per clock.  Tried without gain: stages
+// of 64 bytes in a deeper ring, four waves of 128 x 128, two workgroups of 256 x 128 per CU, wave priorities, a workgroup
+// per CU that walks the tiles and requests the next one's first stages before it stores.
 template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
 __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
     constexpr int WAVES = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
@@ -598,14 +607,14 @@ struct TilePick {
 // fitted to 24 products in all three kinds of type, each timed with every tile and 1 to 64 parts: the cut it takes is at
 // most 1.2 times the fastest (once 1.33), 1.0 in the middle.  Some of those, us, 256 x 256 / 128 x 128 / 128 x 64 / 64 x 64,
 // whole sums, M x N x K: 16-bit 4096 x 250 x 1000 28 / 15 / 11 / 9, 2048 x 2048 x 2048 52 / 31 / 24 / 29, 2048 x 700 x
-// 32000 in 10 parts 98 (128 x 128: 116 in 4); fp32 10007 x 777 x 1004 250 / 196 / 177 / 155; 4-bit 4096 x 4096 x 4096
+// 32000 in 10 parts 98 (128 x 128: 116 in 4); fp32 10007 x 777 x 1004 250 / 196 / 175 / 138; 4-bit 4096 x 4096 x 4096
 // 43 / 47 / 64 / 72, 500 x 200 x 512 13 / 8 / 6 / 5.
 template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, int cus) {
     constexpr bool F32 = std::is_same<T, float>::value, MX4 = std::is_same<T, mx4_t>::value;
     const double rate = F32 ? 0.28e6 : MX4 ? 6.5e6 : 2.1e6, bytes = 45e3;
     // relative to 128 x 128: the large tile draws half the bytes per product, the small ones more
     const struct { int rows, cols; double factor; } kinds[] = {
-        {256, 256, F32 ? 1.0 : MX4 ? 1.23 : 1.33}, {kTile, kTile, 1.0}, {kTile, 64, F32 ? 0.9 : 0.8}, {kTile, 32, F32 ? 0.8 : 0.5}, {64, 64, F32 ? 0.9 : 0.6}};
+        {256, 256, F32 ? 1.0 : MX4 ? 1.23 : 1.33}, {kTile, kTile, 1.0}, {kTile, 64, F32 ? 0.9 : 0.8}, {kTile, 32, F32 ? 0.8 : 0.5}, {64, 64, F32 ? 1.0 : MX4 ? 0.8 : 0.6}};
     const int stages = ceil_div(K, kStageOf<T>);
     TilePick best = {kTile, kTile, 1};
     double least = 1e30;
@@ -638,7 +647,7 @@ template <typename T, int AO, int BO, class Epi>
 inline void tile_launch(const TileArgs& g, const Epi& epi, const TilePick& pick, int cover, hipStream_t s) {
     constexpr int RB = std::is_same<T, mx4_t>::value ? 64 : 128;
     if (pick.rows == 256) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
-    if (pick.rows == 64) return tile_launch_as<T, AO, BO, 64, 64, 2, 2, RB, RB == 64 ? 5 : 3>(g, epi, pick.parts, cover, s);
+    if (pick.rows == 64) return tile_launch_as<T, AO, BO, 64, 64, 2, 2, RB, RB == 64 ? 5 : sizeof(T) == 4 ? 2 : 3>(g, epi, pick.parts, cover, s);
     if constexpr (RB == 128)            // (a 4-bit stage of 32 rows is less than a load per wave)
         if (pick.cols == 32) return tile_launch_as<T, AO, BO, kTile, 32, 4, 1, RB, 4>(g, epi, pick.parts, cover, s);
     if (pick.cols == 64) return tile_launch_as<T, AO, BO, kTile, 64, 4, 1, RB, RB == 64 ? 5 : 3>(g, epi, pick.parts, cover, s);
