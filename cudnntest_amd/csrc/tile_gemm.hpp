@@ -631,7 +631,7 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
             const double mul = (double)rows * cols * k / (rate * kind.factor);
             const double move = (double)(rows + cols) * split * 128 / bytes;
             // one small tile alone on its CU waits for its own loads
-            const double item = std::max(mul, move) * (rows < 256 && items <= cus ? 1.25 : 1.0);
+            const double item = std::max(mul, move) * (rows < 256 && items <= cus ? (rows == kTile ? 1.4 : 1.25) : 1.0);
             const double t = ceil_div(items, cus) * item + (parts > 1 ? 4.0 + (double)parts * M * N * 8 / 4e6 : 0.0);
             if (t < least) {
                 least = t;
