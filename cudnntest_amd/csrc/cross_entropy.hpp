@@ -314,33 +314,53 @@ __global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int
     }
 }
 
-// dbias[v] = scale * sum_t dl[t][v], fp32, rows in a fixed order: 64 classes x 16 groups of rows per workgroup
-template <typename T>
-__global__ __launch_bounds__(1024) void ce_bias_kernel(const T* __restrict__ dl, long pitch, int width, int twin, int rows, int V,
-                                                       const float* __restrict__ scale, T* __restrict__ dbias) {
-    __shared__ float ex[16][64];
-    const int c = threadIdx.x & 63, part = threadIdx.x >> 6;
-    const int v = blockIdx.x * 64 + c;
-    float s = 0.f;
-    if (v < V) {
-        int t = part;
-        for (; t + 112 < rows; t += 128) {                             // eight loads in flight
-            float a[8];
+// dbias[v] = scale * sum_t dl[t][v], fp32, rows in a fixed order: 64 classes x PARTS groups of rows per workgroup
+template <typename T> struct CeBias {
+    const T* dl;
+    long pitch;
+    int width, twin, rows, V;
+    const float* scale;
+    T* dbias;
+    template <int PARTS> __device__ __forceinline__ void run(int block, float* ex) const {
+        const int c = threadIdx.x & 63, part = threadIdx.x >> 6;
+        const int v = block * 64 + c;
+        float s = 0.f;
+        if (v < V) {
+            for (int two = 0; two <= twin; ++two) {
+                const T* at = dl + two * width + v;
+                int t = part;
+                for (; t + 7 * PARTS < rows; t += 8 * PARTS) {         // eight loads in flight
+                    float a[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) a[u] = to_f32(dl[(long)(t + 16 * u) * pitch + v]);
+                    for (int u = 0; u < 8; ++u) a[u] = to_f32(at[(long)(t + PARTS * u) * pitch]);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) s += a[u];
+                    for (int u = 0; u < 8; ++u) s += a[u];
+                }
+                for (; t < rows; t += PARTS) s += to_f32(at[(long)t * pitch]);
+            }
         }
-        for (; t < rows; t += 16) s += to_f32(dl[(long)t * pitch + v]);
-        if (twin)
-            for (t = part; t < rows; t += 16) s += to_f32(dl[(long)t * pitch + width + v]);
-    }
-    ex[part][c] = s;
-    __syncthreads();
-    if (part != 0 || v >= V) return;
+        ex[part * 64 + c] = s;
+        __syncthreads();
+        if (part != 0 || v >= V) return;
 #pragma unroll
-    for (int k = 1; k < 16; ++k) s += ex[k][c];
-    dbias[v] = from_f32<T>(s * (scale ? *scale : 1.f));
+        for (int k = 1; k < PARTS; ++k) s += ex[k * 64 + c];
+        dbias[v] = from_f32<T>(s * (scale ? *scale : 1.f));
+    }
+};
+template <typename T> __global__ __launch_bounds__(1024) void ce_bias_kernel(CeBias<T> b) {
+    __shared__ float ex[1024];
+    b.template run<16>(blockIdx.x, ex);
+}
+
+// Small problems: dx, dw and dbias in one launch.  Each alone leaves most of the chip idle and waits for its own loads (250
+// rows, 1000 classes, D = 4096 in f16: 15.6 + 12.9 + 4.2 us one after the other).
+template <typename T>
+__global__ __launch_bounds__(256, 2) void ce_gradients_kernel(TileArgs gx, TileStore<T> x, int nx, TileArgs gw, TileStore<T> w, int nw, CeBias<T> bias) {
+    __shared__ __align__(1024) char lds[kSmallRing<T> * kTileSlot<T, 64, 64, 128>];
+    const int b = blockIdx.x;
+    if (b < nx) tile_gemm<T, K_OUTER, K_INNER, 64, 64, 2, 2, 128, kSmallRing<T>>(gx, x, b, 0, lds);
+    else if (b < nx + nw) tile_gemm<T, K_OUTER, K_OUTER, 64, 64, 2, 2, 128, kSmallRing<T>>(gw, w, b - nx, 0, lds);
+    else bias.template run<4>(b - nx - nw, reinterpret_cast<float*>(lds));
 }
 
 // 16-bit dl is stored relative to the largest weight: with equal weights (a mean over the rows) the targets' entries are

@@ -23,6 +23,7 @@ struct Plan {
     int rows;                           // of dl: T rounded up to a stage
     int piece;                          // classes per piece (backward)
     bool twin;                          // dl as two 16-bit values
+    bool together;                      // dx, dw and dbias in one launch
     size_t x, w, logits, stats, picked, scale, dl, dx, dw, total;
 };
 
@@ -33,6 +34,7 @@ size_t place(size_t& at, size_t bytes) {
 }
 
 constexpr int kMostParts = 64;
+constexpr int kTogetherTiles = 8;
 
 template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x, const void* w, bool backward) {
     Plan p = {};
@@ -67,6 +69,9 @@ template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x
         if (!p.small) p.logit = tile_pick<E>(p.piece, T, D, 1, cus);
         p.dx_cut = tile_pick<E>(D, T, p.piece * two, kMostParts, cus);
         p.dw_cut = tile_pick<E>(D, p.piece, T * two, kMostParts, cus);
+        // one launch for the gradients while 64 x 64 tiles of both are a few to a CU, and whole sums are the better cut
+        p.together = p.piece == V && p.dx_cut.parts == 1 && p.dw_cut.parts == 1 &&
+                     (long)ceil_div(D, 64) * (ceil_div(T, 64) + ceil_div(V, 64)) <= kTogetherTiles * (long)cus;
         if (p.dx_cut.parts > 1 || p.piece < V) p.dx = place(at, part_bytes(D, T, p.dx_cut.parts));
         if (p.dw_cut.parts > 1) p.dw = place(at, part_bytes(D, p.piece, p.dw_cut.parts));
     }
@@ -199,49 +204,61 @@ template <typename T> struct Call {
                 tile_launch<T, K_INNER, K_INNER>(logits(v0, n), out, p.logit, p.rows, s);
             }
             LAUNCH_CHECK("ce_dl");
-            if (dx) {                   // dx[t][d] (+)= sum_v w[v][d] dl[t][v]
-                TileArgs g = {};
-                g.a = outer<T>(w + (long)v0 * p.pitch_w, p.pitch_w, n);
-                g.b = inner<T>(dl, pitch, T_);
-                g.M = D;
-                g.N = T_;
-                g.K = n;
-                if (p.twin) {           // over dl, then over what it leaves; w from its start again
-                    g.K = (int)round_up(n, kStageOf<T>);
-                    g.passes = 2;
-                    g.a_turn = -(long)g.K * g.a.pitch;
-                    g.b_turn = (width - g.K) * (long)sizeof(T);
-                }
-                if (dx_direct) tile_launch<T, K_OUTER, K_INNER>(g, dx_store, p.dx_cut, T_, s);
-                else tile_launch<T, K_OUTER, K_INNER>(g, TilePart{dx_part, d4, v0 > 0}, p.dx_cut, T_, s);
+            // dx[t][d] (+)= sum_v w[v][d] dl[t][v]
+            TileArgs gx = {};
+            gx.a = outer<T>(w + (long)v0 * p.pitch_w, p.pitch_w, n);
+            gx.b = inner<T>(dl, pitch, T_);
+            gx.M = D;
+            gx.N = T_;
+            gx.K = n;
+            if (p.twin) {               // over dl, then over what it leaves; w from its start again
+                gx.K = (int)round_up(n, kStageOf<T>);
+                gx.passes = 2;
+                gx.a_turn = -(long)gx.K * gx.a.pitch;
+                gx.b_turn = (width - gx.K) * (long)sizeof(T);
+            }
+            // dw[v][d] = sum_t x[t][d] dl[t][v]
+            TileArgs gw = {};
+            gw.a = outer<T>(x, p.pitch_x, T_);
+            gw.b = outer<T>(dl, pitch, p.rows);
+            gw.M = D;
+            gw.N = n;
+            gw.K = T_;
+            if (p.twin) {
+                gw.K = p.rows;
+                gw.passes = 2;
+                gw.a_turn = -(long)gw.K * gw.a.pitch;
+                gw.b_turn = -(long)gw.K * gw.b.pitch + width * (long)sizeof(T);
+            }
+            const TileStore<T> dw_store = {dw ? dw + (long)v0 * D : nullptr, D, nullptr, back, 0};
+            const CeBias<T> bias_sum = {dl, pitch, width, p.twin, T_, n, back, dbias ? dbias + v0 : nullptr};
+            if (p.together && dx && dw) {
+                tile_prepare<T, K_OUTER, K_INNER, 64, 64, 128>(gx, 1, T_);
+                tile_prepare<T, K_OUTER, K_OUTER, 64, 64, 128>(gw, 1, n);
+                const int nx = tile_grid(gx.mt, gx.nt), nw = tile_grid(gw.mt, gw.nt);
+                hipLaunchKernelGGL((ce_gradients_kernel<T>), dim3(nx + nw + (dbias ? ceil_div(n, 64) : 0)), dim3(256), 0, s, gx, dx_store, nx, gw,
+                                   dw_store, nw, bias_sum);
+                LAUNCH_CHECK("ce_gradients");
+                return WINO_OK;
+            }
+            if (dx) {
+                if (dx_direct) tile_launch<T, K_OUTER, K_INNER>(gx, dx_store, p.dx_cut, T_, s);
+                else tile_launch<T, K_OUTER, K_INNER>(gx, TilePart{dx_part, d4, v0 > 0}, p.dx_cut, T_, s);
                 LAUNCH_CHECK("ce_dx");
             }
-            if (dw) {                   // dw[v][d] = sum_t x[t][d] dl[t][v]
-                TileArgs g = {};
-                g.a = outer<T>(x, p.pitch_x, T_);
-                g.b = outer<T>(dl, pitch, p.rows);
-                g.M = D;
-                g.N = n;
-                g.K = T_;
-                if (p.twin) {
-                    g.K = p.rows;
-                    g.passes = 2;
-                    g.a_turn = -(long)g.K * g.a.pitch;
-                    g.b_turn = -(long)g.K * g.b.pitch + width * (long)sizeof(T);
-                }
-                const TileStore<T> store = {dw + (long)v0 * D, D, nullptr, back, 0};
+            if (dw) {
                 if (p.dw_cut.parts == 1) {
-                    tile_launch<T, K_OUTER, K_OUTER>(g, store, p.dw_cut, n, s);
+                    tile_launch<T, K_OUTER, K_OUTER>(gw, dw_store, p.dw_cut, n, s);
                 } else {
-                    tile_launch<T, K_OUTER, K_OUTER>(g, TilePart{dw_part, d4, 0}, p.dw_cut, n, s);
+                    tile_launch<T, K_OUTER, K_OUTER>(gw, TilePart{dw_part, d4, 0}, p.dw_cut, n, s);
                     LAUNCH_CHECK("ce_dw");
                     hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(D, 4) * n, 256)), dim3(256), 0, s,
-                                       dw_part, p.dw_cut.parts, d4, D, n, store);
+                                       dw_part, p.dw_cut.parts, d4, D, n, dw_store);
                 }
                 LAUNCH_CHECK("ce_dw");
             }
             if (dbias) {
-                hipLaunchKernelGGL((ce_bias_kernel<T>), dim3(ceil_div(n, 64)), dim3(1024), 0, s, dl, pitch, width, p.twin, T_, n, back, dbias + v0);
+                hipLaunchKernelGGL((ce_bias_kernel<T>), dim3(ceil_div(n, 64)), dim3(1024), 0, s, bias_sum);
                 LAUNCH_CHECK("ce_bias");
             }
         }

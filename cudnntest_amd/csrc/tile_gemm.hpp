@@ -213,28 +213,29 @@ inline int tile_grid(int mt, int nt) { return (mt * nt + 7) / 8 * 8; }
 // clock follows the data).  4-bit 4096 x 8192 x 8192: 155 us, 3.5 PFLOP/s, the same bytes per clock.  Tried without gain: stages
 // of 64 bytes in a deeper ring, four waves of 128 x 128, two workgroups of 256 x 128 per CU, wave priorities, a workgroup
 // per CU that walks the tiles and requests the next one's first stages before it stores.
+template <typename T, int BM, int BN, int RB> constexpr int kTileSlot =       // LDS of a stage; 4-bit scales 1 KB at a time
+    (BM + BN) * RB + (std::is_same<T, mx4_t>::value ? ((BM * RB / 16 + 1023) / 1024 + (BN * RB / 16 + 1023) / 1024) * 1024 : 0);
+
+// one tile (or part `part` of its reduction): `id` counts the tiles, lds holds RING stages
 template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
+__device__ __forceinline__ void tile_gemm(const TileArgs& g, const Epi& epi, int id, int part, char* lds) {
     constexpr int WAVES = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32;
     constexpr bool MX4 = std::is_same<T, mx4_t>::value;
     constexpr int STAGE = RB / 16 * TileElem<T>::piece, STEPS = RB / 32;   // elements of k, multiplies of a lane half
     typedef TileSide<T, AO, BM, WAVES, RB> SA;
     typedef TileSide<T, BO, BN, WAVES, RB> SB;
-    // scale bytes of a stage: one per piece, loaded 1 KB at a time
-    constexpr int SROW = RB / 16, SCA = (BM * SROW + 1023) / 1024, SCB = (BN * SROW + 1023) / 1024;
-    constexpr int SC = MX4 ? (SCA + SCB) * 1024 : 0;
-    constexpr int SLOT = SA::kBytes + SB::kBytes + SC;
+    constexpr int SROW = RB / 16, SCA = (BM * SROW + 1023) / 1024, SCB = (BN * SROW + 1023) / 1024;      // scale bytes, loads
+    constexpr int SLOT = kTileSlot<T, BM, BN, RB>;
     constexpr bool TWO = AO == K_OUTER && sizeof(T) == 2;              // the products that run in two passes
-    __shared__ __align__(1024) char lds[RING * SLOT];
 
     int tm, tn;
-    if (!tile_of(blockIdx.x, g.mt, g.nt, tm, tn)) return;
+    if (!tile_of(id, g.mt, g.nt, tm, tn)) return;
     const int m0 = tm * BM, n0 = tn * BN;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
     const int l32 = lane & 31, lh = lane >> 5;
-    const int first = blockIdx.y * g.split, last = min(first + g.split, g.stages);
+    const int first = part * g.split, last = min(first + g.split, g.stages);
 
     SA sa;
     SB sb;
@@ -412,6 +413,12 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_k
     epi.template run<BM, BN, WM, WN, MI, NI>(acc, g, m0, n0, wm, wn, l32, lh, lds);
 }
 
+template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN > 4 ? 1 : 2) void tile_gemm_kernel(TileArgs g, Epi epi) {
+    __shared__ __align__(1024) char lds[RING * kTileSlot<T, BM, BN, RB>];
+    tile_gemm<T, AO, BO, BM, BN, WM, WN, RB, RING>(g, epi, blockIdx.x, blockIdx.y, lds);
+}
+
 // ---- epilogues ---------------------------------------------------------------------------------
 
 // four consecutive elements of an output row; vec: the row and its base allow one store
@@ -576,8 +583,8 @@ constexpr int kTile = 128;               // edge of the usual tile
 
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
-inline void tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hipStream_t s) {
+// the fields of g that follow from the tile and the parts; returns the parts that are not empty
+template <typename T, int AO, int BO, int BM, int BN, int RB> inline int tile_prepare(TileArgs& g, int parts, int cover) {
     g.mt = ceil_div(g.M, BM);
     g.nt = ceil_div(cover, BN);
     constexpr int stage = RB / 16 * TileElem<T>::piece;
@@ -590,12 +597,19 @@ inline void tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hip
     g.tail_at = g.passes > 1 ? (AO == K_OUTER && g.a.rows < g.K ? g.pass - 1 : -1) : g.K % stage ? g.pass - 1 : -1;
     g.stages = g.passes * g.pass;
     g.split = ceil_div(g.stages, parts);
-    parts = ceil_div(g.stages, g.split);
+    return ceil_div(g.stages, g.split);
+}
+
+template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
+inline void tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hipStream_t s) {
+    parts = tile_prepare<T, AO, BO, BM, BN, RB>(g, parts, cover);
     hipLaunchKernelGGL((tile_gemm_kernel<T, AO, BO, BM, BN, WM, WN, RB, RING, Epi>), dim3(tile_grid(g.mt, g.nt), parts), dim3(64 * WM * WN), 0, s, g, epi);
 }
 
-// How a product is cut: the tile (256 x 256, or 128 x cols) and the parts of its reduction.
 template <typename T> constexpr int kStageOf = 8 * TileElem<T>::piece;     // elements of k in 128 bytes
+
+// stages in LDS of a 64 x 64 tile: fp32 is bound by its multiplies and takes more workgroups to a CU instead
+template <typename T> constexpr int kSmallRing = std::is_same<T, mx4_t>::value ? 5 : sizeof(T) == 4 ? 2 : 3;
 
 struct TilePick {
     int rows, cols, parts;      // m and n extent of a tile, parts of the reduction
@@ -647,7 +661,7 @@ template <typename T, int AO, int BO, class Epi>
 inline void tile_launch(const TileArgs& g, const Epi& epi, const TilePick& pick, int cover, hipStream_t s) {
     constexpr int RB = std::is_same<T, mx4_t>::value ? 64 : 128;
     if (pick.rows == 256) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
-    if (pick.rows == 64) return tile_launch_as<T, AO, BO, 64, 64, 2, 2, RB, RB == 64 ? 5 : sizeof(T) == 4 ? 2 : 3>(g, epi, pick.parts, cover, s);
+    if (pick.rows == 64) return tile_launch_as<T, AO, BO, 64, 64, 2, 2, RB, kSmallRing<T>>(g, epi, pick.parts, cover, s);
     if constexpr (RB == 128)            // (a 4-bit stage of 32 rows is less than a load per wave)
         if (pick.cols == 32) return tile_launch_as<T, AO, BO, kTile, 32, 4, 1, RB, 4>(g, epi, pick.parts, cover, s);
     if (pick.cols == 64) return tile_launch_as<T, AO, BO, kTile, 64, 4, 1, RB, RB == 64 ? 5 : 3>(g, epi, pick.parts, cover, s);
