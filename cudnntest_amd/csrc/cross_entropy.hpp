@@ -286,9 +286,81 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(CeParts<T> p, CeRows rows
     loss[t] = target == rows.ignore ? 0.f : target < 0 || target >= rows.V ? NAN : z - picked;
 }
 
-// small problems: dl from the partial sums, four classes per thread
+// 16-bit dl is stored relative to the largest weight: with equal weights (a mean over the rows) the targets' entries are
+// then close to -1, which the type holds well, instead of all sharing the rounding error of the weight.  f16 in addition
+// has only five exponent bits: times 2^15 (|exp(l - lse) - hit| <= 1, so nothing overflows), which keeps values down to
+// 2^-39 of the largest weight.  `top` is 1 or 2^15; the factor is top / weight_top(), its inverse is applied to the fp32
+// sums.  Called by a whole workgroup; ex holds one float per wave.
+__device__ __forceinline__ float weight_top(const float* grad, const CeRows& rows, int T, float top, float* ex) {
+    float mx = 0.f;
+    for (int t = threadIdx.x; t < T; t += blockDim.x)
+        if (rows.target[t] != rows.ignore) mx = fmaxf(mx, fabsf(grad[t]));
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
+    if ((threadIdx.x & 63) == 0) ex[threadIdx.x >> 6] = mx;
+    __syncthreads();
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) mx = fmaxf(mx, ex[w]);
+    // no weight at all, or none that is finite: factor 1
+    return mx > 0.f && mx <= 3.4028235e38f ? fmaxf(mx, 1e-30f) : top;
+}
+// out[0] = the factor, out[1] = its inverse
+__global__ __launch_bounds__(1024) static void ce_scale_kernel(const float* __restrict__ grad, CeRows rows, int T, float top, float* __restrict__ out) {
+    __shared__ float ex[16];
+    const float g = weight_top(grad, rows, T, top, ex);
+    if (threadIdx.x != 0) return;
+    out[0] = top / g;
+    out[1] = g / top;
+}
+
+// Rows copied to a 16-byte aligned pitch, zeros behind them, and in place of rows whose target is `ignore` (target null:
+// none).  Backward reads x through such a copy: an ignored row's dl is zero, but zero times what an unused row of a padded
+// batch may hold (a NaN, an infinity) would still reach every class's dw.
+template <typename T> struct RowCopy {
+    const T* x;
+    T* y;
+    long rows;
+    int cols, pitch;                    // elements; y's pitch is a multiple of 16 bytes
+    const long long* target;
+    long long ignore;
+    static constexpr int kPer = 16 / (int)sizeof(T);
+    long blocks() const { return (rows * (pitch / kPer) + 255) / 256; }
+    __device__ __forceinline__ void run(long block) const {
+        const long i = block * 256 + threadIdx.x;
+        const int pieces = pitch / kPer;
+        const long row = i / pieces;
+        if (row >= rows) return;
+        const int c = (int)(i - row * pieces) * kPer;
+        const T* from = x + row * cols + c;
+        Pack16<T> pk;
+        const bool keep = !target || target[row] != ignore;
+        if (cols == pitch && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
+            pk = *reinterpret_cast<const Pack16<T>*>(from);
+            if (!keep) pk = __builtin_bit_cast(Pack16<T>, uintx4{0, 0, 0, 0});
+        } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) pk.e[e] = keep && c + e < cols ? from[e] : from_f32<T>(0.f);
+        }
+        *reinterpret_cast<Pack16<T>*>(y + row * pitch + c) = pk;
+    }
+};
+template <typename T> __global__ __launch_bounds__(256) void row_copy_kernel(RowCopy<T> c) { c.run(blockIdx.x); }
+
+// small problems: dl from the partial sums, four classes per thread.  scale: null, or where the factor and its inverse go
+// (every workgroup finds them itself, which saves a launch)
 template <typename T>
-__global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int T_rows) {
+__global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int T_rows, float top, float* __restrict__ scale, int blocks,
+                                                    RowCopy<T> copy) {
+    __shared__ float ex[4];
+    if ((int)blockIdx.x >= blocks) return copy.run(blockIdx.x - blocks);        // beside dl: x for dw
+    float f = o.scale ? *o.scale : 1.f;
+    if (scale) {
+        const float g = weight_top(o.grad, o.rows, T_rows, top, ex);
+        f = top / g;
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            scale[0] = f;
+            scale[1] = g / top;
+        }
+    }
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
     const int quads = o.width / 4;
     const int t = (int)(i / quads), m = (int)(i - (long)t * quads) * 4;
@@ -296,7 +368,7 @@ __global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int
     const bool in = t < T_rows;
     const long long target = in ? o.rows.target[t] : o.rows.ignore;
     const bool ignored = !in || target == o.rows.ignore;
-    const float weight = in ? row_weight(o.rows, target, o.grad[t]) * (o.scale ? *o.scale : 1.f) : 0.f;
+    const float weight = in ? row_weight(o.rows, target, o.grad[t]) * f : 0.f;
     const float z = in ? o.lse[t] : 0.f;
     floatx4 l = {0.f, 0.f, 0.f, 0.f};
     if (in && m < o.rows.V) l = sum_parts<floatx4>(p.part + t * p.pitch + m, p.parts, p.plane);              // m + 3 < pitch of the parts
@@ -314,89 +386,53 @@ __global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int
     }
 }
 
-// dbias[v] = scale * sum_t dl[t][v], fp32, rows in a fixed order: 64 classes x PARTS groups of rows per workgroup
+// dbias[v] = scale * sum_t dl[t][v], fp32: 64 classes per workgroup, 16 groups of rows shared by its waves and added in order
 template <typename T> struct CeBias {
     const T* dl;
     long pitch;
     int width, twin, rows, V;
     const float* scale;
     T* dbias;
-    template <int PARTS> __device__ __forceinline__ void run(int block, float* ex) const {
-        const int c = threadIdx.x & 63, part = threadIdx.x >> 6;
-        const int v = block * 64 + c;
-        float s = 0.f;
-        if (v < V) {
-            for (int two = 0; two <= twin; ++two) {
+    __device__ __forceinline__ void run(int block, float* ex) const {  // ex [16][64]
+        const int c = threadIdx.x & 63, v = block * 64 + c, waves = blockDim.x >> 6;
+        for (int g = threadIdx.x >> 6; g < 16; g += waves) {
+            float s = 0.f;
+            for (int two = 0; v < V && two <= twin; ++two) {
                 const T* at = dl + two * width + v;
-                int t = part;
-                for (; t + 7 * PARTS < rows; t += 8 * PARTS) {         // eight loads in flight
+                int t = g;
+                for (; t + 112 < rows; t += 128) {                     // eight loads in flight
                     float a[8];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) a[u] = to_f32(at[(long)(t + PARTS * u) * pitch]);
+                    for (int u = 0; u < 8; ++u) a[u] = to_f32(at[(long)(t + 16 * u) * pitch]);
 #pragma unroll
                     for (int u = 0; u < 8; ++u) s += a[u];
                 }
-                for (; t < rows; t += PARTS) s += to_f32(at[(long)t * pitch]);
+                for (; t < rows; t += 16) s += to_f32(at[(long)t * pitch]);
             }
+            ex[g * 64 + c] = s;
         }
-        ex[part * 64 + c] = s;
         __syncthreads();
-        if (part != 0 || v >= V) return;
+        if (threadIdx.x >= 64 || v >= V) return;
+        float s = ex[c];
 #pragma unroll
-        for (int k = 1; k < PARTS; ++k) s += ex[k * 64 + c];
+        for (int g = 1; g < 16; ++g) s += ex[g * 64 + c];
         dbias[v] = from_f32<T>(s * (scale ? *scale : 1.f));
     }
 };
 template <typename T> __global__ __launch_bounds__(1024) void ce_bias_kernel(CeBias<T> b) {
     __shared__ float ex[1024];
-    b.template run<16>(blockIdx.x, ex);
+    b.run(blockIdx.x, ex);
 }
 
 // Small problems: dx, dw and dbias in one launch.  Each alone leaves most of the chip idle and waits for its own loads (250
-// rows, 1000 classes, D = 4096 in f16: 15.6 + 12.9 + 4.2 us one after the other).
+// rows, 1000 classes, D = 4096 in f16: 15.6 + 12.9 + 4.2 us one after the other, 21.7 together).
 template <typename T>
-__global__ __launch_bounds__(256, 2) void ce_gradients_kernel(TileArgs gx, TileStore<T> x, int nx, TileArgs gw, TileStore<T> w, int nw, CeBias<T> bias) {
+__global__ __launch_bounds__(256, 2) void ce_gradients_kernel(CeBias<T> bias, int nb, TileArgs gx, TileStore<T> x, int nx, TileArgs gw, TileStore<T> w) {
     __shared__ __align__(1024) char lds[kSmallRing<T> * kTileSlot<T, 64, 64, 128>];
     const int b = blockIdx.x;
-    if (b < nx) tile_gemm<T, K_OUTER, K_INNER, 64, 64, 2, 2, 128, kSmallRing<T>>(gx, x, b, 0, lds);
-    else if (b < nx + nw) tile_gemm<T, K_OUTER, K_OUTER, 64, 64, 2, 2, 128, kSmallRing<T>>(gw, w, b - nx, 0, lds);
-    else bias.template run<4>(b - nx - nw, reinterpret_cast<float*>(lds));
-}
-
-// 16-bit dl is stored relative to the largest weight: with equal weights (a mean over the rows) the targets' entries are
-// then close to -1, which the type holds well, instead of all sharing the rounding error of the weight.  f16 in addition
-// has only five exponent bits: times 2^15 (|exp(l - lse) - hit| <= 1, so nothing overflows), which keeps values down to
-// 2^-39 of the largest weight.  out[0] = the factor, out[1] = its inverse, applied to the fp32 sums.
-__global__ __launch_bounds__(1024) static void ce_scale_kernel(const float* __restrict__ grad, CeRows rows, int T, float top, float* __restrict__ out) {
-    __shared__ float ex[1024];
-    float mx = 0.f;
-    for (int t = threadIdx.x; t < T; t += 1024)
-        if (rows.target[t] != rows.ignore) mx = fmaxf(mx, fabsf(grad[t]));
-    ex[threadIdx.x] = mx;
-    __syncthreads();
-    for (int k = 512; k > 0; k >>= 1) {
-        if ((int)threadIdx.x < k) ex[threadIdx.x] = fmaxf(ex[threadIdx.x], ex[threadIdx.x + k]);
-        __syncthreads();
-    }
-    if (threadIdx.x != 0) return;
-    // no weight at all, or none that is finite: 1
-    const float g = ex[0] > 0.f && ex[0] <= 3.4028235e38f ? fmaxf(ex[0], 1e-30f) : top;
-    out[0] = top / g;
-    out[1] = g / top;
-}
-
-// rows of `cols` elements copied to a 16-byte aligned pitch, zeros behind them
-template <typename T>
-__global__ __launch_bounds__(256) void pad_rows_kernel(const T* __restrict__ x, long rows, int cols, T* __restrict__ y, int pitch) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    const int quads = pitch / 4;
-    const long row = i / quads;
-    if (row >= rows) return;
-    const int c = (int)(i - row * quads) * 4;
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = c + e < cols ? to_f32(x[row * cols + c + e]) : 0.f;
-    store4<T>(y + row * pitch + c, v, 4, true);
+    if (b < nb) bias.run(b, reinterpret_cast<float*>(lds));            // (the longest wait first)
+    else if (b < nb + nx) tile_gemm<T, K_OUTER, K_INNER, 64, 64, 2, 2, 128, kSmallRing<T>>(gx, x, b - nb, 0, lds);
+    else tile_gemm<T, K_OUTER, K_OUTER, 64, 64, 2, 2, 128, kSmallRing<T>>(gw, w, b - nb - nx, 0, lds);
 }
 
 }  // namespace wino

@@ -16,7 +16,7 @@ constexpr size_t kPieceBytes = 128u << 20;            // dl of one piece of the 
 // Where everything is in the workspace, and how the problem is cut.  The same function sizes the workspace and drives
 // the calls.
 struct Plan {
-    bool pad_x, pad_w;                  // copied to 16-byte aligned rows first (odd lengths or bases)
+    bool pad_x, pad_w;                  // copied to 16-byte aligned rows first (odd lengths or bases); backward copies x for dw anyway
     int pitch_x, pitch_w;               // elements
     bool small;                         // too few tiles for the chip: logits as partial sums of a cut reduction
     TilePick logit, dx_cut, dw_cut;     // how the three products are cut
@@ -52,7 +52,7 @@ template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x
     const int two = p.twin ? 2 : 1;
     p.small = p.logit.parts > 1 && (!backward || (size_t)p.rows * round_up(V, 128) * e * two <= kPieceBytes);
     size_t at = 0;
-    if (p.pad_x) p.x = place(at, (size_t)T * p.pitch_x * e);
+    if (p.pad_x || backward) p.x = place(at, (size_t)T * p.pitch_x * e);
     if (p.pad_w) p.w = place(at, (size_t)V * p.pitch_w * e);
     if (p.small) p.logits = place(at, part_bytes(V, T, p.logit.parts));
     else p.logit = tile_pick<E>(V, T, D, 1, cus);
@@ -107,11 +107,10 @@ template <typename T> TileOperand outer(const T* p, long pitch, int k_rows) {
     return {reinterpret_cast<const char*>(p), nullptr, b, 0, k_rows, (int)(b / 16)};
 }
 
-template <typename T> int pad_rows(const T* x, long rows, int cols, T* y, int pitch, hipStream_t s) {
-    const long n = rows * (pitch / 4);
-    if (n / 256 > 0x7ffffff0L) return fail(WINO_ERR_UNSUPPORTED, "pad_rows: %ld rows of %d", rows, cols);
-    hipLaunchKernelGGL((pad_rows_kernel<T>), dim3(ceil_div(n, 256)), dim3(256), 0, s, x, rows, cols, y, pitch);
-    LAUNCH_CHECK("pad_rows");
+template <typename T> int row_copy(const RowCopy<T>& c, hipStream_t s) {
+    if (c.blocks() > 0x7ffffff0L) return fail(WINO_ERR_UNSUPPORTED, "row copy: %ld rows of %d", c.rows, c.cols);
+    hipLaunchKernelGGL((row_copy_kernel<T>), dim3((unsigned)c.blocks()), dim3(256), 0, s, c);
+    LAUNCH_CHECK("row_copy");
     return WINO_OK;
 }
 
@@ -123,18 +122,22 @@ template <typename T> struct Call {
     char* ws;
     hipStream_t s;
 
-    int operands() {
+    // backward: without what ignored rows hold
+    RowCopy<T> copy_of_x(bool backward) const {
+        return {x, reinterpret_cast<T*>(ws + p.x), T_, D, p.pitch_x, backward ? rows.target : nullptr, rows.ignore};
+    }
+    int operands(bool backward) {
         if (p.pad_x) {
-            T* y = reinterpret_cast<T*>(ws + p.x);
-            const int rc = pad_rows<T>(x, T_, D, y, p.pitch_x, s);
+            const RowCopy<T> c = copy_of_x(backward);
+            const int rc = row_copy<T>(c, s);
             if (rc) return rc;
-            x = y;
+            x = c.y;
         }
         if (p.pad_w) {
-            T* y = reinterpret_cast<T*>(ws + p.w);
-            const int rc = pad_rows<T>(w, V, D, y, p.pitch_w, s);
+            const RowCopy<T> c = {w, reinterpret_cast<T*>(ws + p.w), V, D, p.pitch_w, nullptr, 0};
+            const int rc = row_copy<T>(c, s);
             if (rc) return rc;
-            w = y;
+            w = c.y;
         }
         return WINO_OK;
     }
@@ -157,7 +160,7 @@ template <typename T> struct Call {
     }
 
     int forward(float* loss, float* lse) {
-        int rc = operands();
+        int rc = operands(false);
         if (rc) return rc;
         if (p.small) {
             CeParts<T> parts;
@@ -176,13 +179,22 @@ template <typename T> struct Call {
     }
 
     int backward(const float* grad, const float* lse, T* dx, T* dw, T* dbias) {
-        int rc = operands();
+        int rc = operands(true);
         if (rc) return rc;
+        // x for dw: copied with the operands, by the kernel that writes a small problem's dl, or here
+        RowCopy<T> copy = copy_of_x(true);
+        const bool copy_inside = p.small && dw && !p.pad_x && copy.blocks() < (1 << 20);
+        if (dw && !p.pad_x && !copy_inside && (rc = row_copy<T>(copy, s))) return rc;
+        const T* xw = copy.y;
         float* scale = nullptr;
+        const float top = std::is_same<T, f16_t>::value ? 32768.f : 1.f;
+        const bool scale_inside = p.small && T_ <= 1024;      // the kernel that writes dl finds the factor itself
         if (sizeof(T) == 2) {
             scale = reinterpret_cast<float*>(ws + p.scale);
-            hipLaunchKernelGGL(ce_scale_kernel, dim3(1), dim3(1024), 0, s, grad, rows, T_, std::is_same<T, f16_t>::value ? 32768.f : 1.f, scale);
-            LAUNCH_CHECK("ce_scale");
+            if (!scale_inside) {
+                hipLaunchKernelGGL(ce_scale_kernel, dim3(1), dim3(1024), 0, s, grad, rows, T_, top, scale);
+                LAUNCH_CHECK("ce_scale");
+            }
         }
         const float* back = scale ? scale + 1 : nullptr;
         T* dl = reinterpret_cast<T*>(ws + p.dl);
@@ -195,11 +207,13 @@ template <typename T> struct Call {
             const int n = std::min(p.piece, V - v0);
             const int width = (int)round_up(n, 128);
             const long pitch = p.twin ? 2L * width : width;
-            const CeDl<T> out = {bias ? bias + v0 : nullptr, rows, lse, grad, scale, v0, dl, pitch, width, p.rows, p.twin};
+            const CeDl<T> out = {bias ? bias + v0 : nullptr, rows, lse, grad, scale_inside ? nullptr : scale, v0, dl, pitch, width, p.rows, p.twin};
             if (p.small) {
                 CeParts<T> parts;
                 if ((rc = partial_logits(&parts))) return rc;
-                hipLaunchKernelGGL((ce_dl_kernel<T>), dim3(ceil_div((long)p.rows * (width / 4), 256)), dim3(256), 0, s, parts, out, T_);
+                const int blocks = ceil_div((long)p.rows * (width / 4), 256);
+                hipLaunchKernelGGL((ce_dl_kernel<T>), dim3(blocks + (copy_inside ? (int)copy.blocks() : 0)), dim3(256), 0, s, parts, out, T_, top,
+                                   scale_inside ? scale : nullptr, blocks, copy);
             } else {
                 tile_launch<T, K_INNER, K_INNER>(logits(v0, n), out, p.logit, p.rows, s);
             }
@@ -219,7 +233,7 @@ template <typename T> struct Call {
             }
             // dw[v][d] = sum_t x[t][d] dl[t][v]
             TileArgs gw = {};
-            gw.a = outer<T>(x, p.pitch_x, T_);
+            gw.a = outer<T>(xw, p.pitch_x, T_);
             gw.b = outer<T>(dl, pitch, p.rows);
             gw.M = D;
             gw.N = n;
@@ -236,8 +250,8 @@ template <typename T> struct Call {
                 tile_prepare<T, K_OUTER, K_INNER, 64, 64, 128>(gx, 1, T_);
                 tile_prepare<T, K_OUTER, K_OUTER, 64, 64, 128>(gw, 1, n);
                 const int nx = tile_grid(gx.mt, gx.nt), nw = tile_grid(gw.mt, gw.nt);
-                hipLaunchKernelGGL((ce_gradients_kernel<T>), dim3(nx + nw + (dbias ? ceil_div(n, 64) : 0)), dim3(256), 0, s, gx, dx_store, nx, gw,
-                                   dw_store, nw, bias_sum);
+                const int nb = dbias ? (ceil_div(n, 64) + 7) / 8 * 8 : 0;      // (the tiles keep their XCDs)
+                hipLaunchKernelGGL((ce_gradients_kernel<T>), dim3(nb + nx + nw), dim3(256), 0, s, bias_sum, nb, gx, dx_store, nx, gw, dw_store);
                 LAUNCH_CHECK("ce_gradients");
                 return WINO_OK;
             }

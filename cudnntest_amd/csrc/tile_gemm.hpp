@@ -628,7 +628,7 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
     const double rate = F32 ? 0.28e6 : MX4 ? 6.5e6 : 2.1e6, bytes = 45e3;
     // relative to 128 x 128: the large tile draws half the bytes per product, the small ones more
     const struct { int rows, cols; double factor; } kinds[] = {
-        {256, 256, F32 ? 1.0 : MX4 ? 1.23 : 1.33}, {kTile, kTile, 1.0}, {kTile, 64, F32 ? 0.9 : 0.8}, {kTile, 32, F32 ? 0.8 : 0.5}, {64, 64, F32 ? 1.0 : MX4 ? 0.8 : 0.6}};
+        {256, 256, F32 ? 1.0 : MX4 ? 1.23 : 1.33}, {kTile, kTile, 1.0}, {kTile, 64, F32 ? 0.9 : 0.8}, {kTile, 32, F32 ? 1.05 : 0.5}, {64, 64, F32 ? 1.0 : MX4 ? 0.8 : 0.6}};
     const int stages = ceil_div(K, kStageOf<T>);
     TilePick best = {kTile, kTile, 1};
     double least = 1e30;

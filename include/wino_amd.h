@@ -354,7 +354,8 @@ int wino_mx4_linear(int dtype, unsigned flags, int M, int N, int K, const void *
  * ignore_index makes the row's loss NaN.  Logits of -infinity (from the bias) mask their class; a row in which they all are
  * has lse -infinity and loss NaN; a logit that is NaN or +infinity makes its row NaN.
  * x and w are read in place when their rows are 16-byte aligned (D times the element size and both base addresses), and
- * copied to aligned rows in the workspace otherwise: the workspace query takes the addresses of the call to come. */
+ * copied to aligned rows in the workspace otherwise: the workspace query takes the addresses of the call to come.  What an
+ * ignored row of x holds (NaNs, infinities) reaches its own lse and nothing else. */
 size_t wino_linear_cross_entropy_workspace_bytes(int dtype, int T, int D, int V, const void *x, const void *w, int backward);
 int wino_linear_cross_entropy(int dtype, int T, int D, int V, const void *x, const void *w, const void *bias,
                               const long long *target, long long ignore_index, float *loss, float *lse, void *workspace,

@@ -110,7 +110,6 @@ def test_all_rows_ignored(T, V):
     assert bool((loss == 0).all()) and bool(torch.isfinite(lse).all())
     x[0, 0] = NAN                                          # an ignored row's NaN goes nowhere but into its own lse
     _, lse = ops.linear_cross_entropy(x, w, target, bias=b, ignore_index=7)
-    x[0, 0] = 0.0
     for g in ops.linear_cross_entropy_backward(grad, x, w, target, lse, bias=b, ignore_index=7):
         assert bool((g == 0).all())
 
@@ -290,3 +289,22 @@ def test_two_streams_and_threads_at_once():
         assert len(got[k]) == 8
         for out in got[k]:
             assert all(torch.equal(a, c) for a, c in zip(out, want[k]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,D,V", [(40, 64, 100), (130, 33, 500), (300, 64, 400), (700, 64, 9000), (1, 64, 50)])
+def test_what_ignored_rows_hold_reaches_nothing(T, D, V, dtype):
+    """A padded batch: rows behind the last one hold NaN, infinities, garbage weights and are ignored."""
+    x, w, target, b, grad = problem(T, D, V, dtype, ignore=False)
+    off = torch.zeros(T, dtype=torch.bool, device="cuda")
+    off[::3] = True
+    off[-1] = True                                         # the last row, which also fills the reduction's last stage
+    target[off] = -100
+    want = ops.linear_cross_entropy(x, w, target, bias=b)
+    want += ops.linear_cross_entropy_backward(grad, x, w, target, want[1], bias=b)
+    x[off], grad[off] = NAN, INF
+    x[-1, 0] = -INF
+    loss, lse = ops.linear_cross_entropy(x, w, target, bias=b)
+    assert torch.equal(loss, want[0]) and torch.equal(lse[~off], want[1][~off]) and bool(torch.isnan(lse[off]).all())
+    for got, ref in zip(ops.linear_cross_entropy_backward(grad, x, w, target, lse, bias=b), want[2:]):
+        assert torch.equal(got, ref)
