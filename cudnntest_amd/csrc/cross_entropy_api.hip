@@ -67,8 +67,9 @@ template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x
         p.piece = p.small ? V : (int)std::min<size_t>(V, std::max<size_t>(fit, 256));
         p.dl = place(at, (size_t)p.rows * round_up(p.piece, 128) * e * two);
         if (!p.small) p.logit = tile_pick<E>(p.piece, T, D, 1, cus);
-        p.dx_cut = tile_pick<E>(D, T, p.piece * two, kMostParts, cus);
-        p.dw_cut = tile_pick<E>(D, p.piece, T * two, kMostParts, cus);
+        // the reductions as they run: twice over whole stages where dl is two values (the join adds as many parts as the cut has)
+        p.dx_cut = tile_pick<E>(D, T, p.twin ? 2 * (int)round_up(p.piece, kStageOf<E>) : p.piece, kMostParts, cus);
+        p.dw_cut = tile_pick<E>(D, p.piece, p.twin ? 2 * p.rows : T, kMostParts, cus);
         // one launch for the gradients while 64 x 64 tiles of both are a few to a CU, and whole sums are the better cut
         p.together = p.piece == V && p.dx_cut.parts == 1 && p.dw_cut.parts == 1 &&
                      (long)ceil_div(D, 64) * (ceil_div(T, 64) + ceil_div(V, 64)) <= kTogetherTiles * (long)cus;
@@ -153,8 +154,9 @@ template <typename T> struct Call {
     int partial_logits(CeParts<T>* parts) {
         float* to = reinterpret_cast<float*>(ws + p.logits);
         const long pitch = round_up(V, 4);
-        tile_launch<T, K_INNER, K_INNER>(logits(0, V), TilePart{to, pitch, 0}, p.logit, T_, s);
+        const int made = tile_launch<T, K_INNER, K_INNER>(logits(0, V), TilePart{to, pitch, 0}, p.logit, T_, s);
         LAUNCH_CHECK("logits in parts");
+        if (made != p.logit.parts) return fail(WINO_ERR_HIP, "logits: %d parts for %d", made, p.logit.parts);
         *parts = {to, p.logit.parts, pitch, pitch * T_, bias};
         return WINO_OK;
     }
@@ -256,16 +258,20 @@ template <typename T> struct Call {
                 return WINO_OK;
             }
             if (dx) {
+                int made = p.dx_cut.parts;
                 if (dx_direct) tile_launch<T, K_OUTER, K_INNER>(gx, dx_store, p.dx_cut, T_, s);
-                else tile_launch<T, K_OUTER, K_INNER>(gx, TilePart{dx_part, d4, v0 > 0}, p.dx_cut, T_, s);
+                else made = tile_launch<T, K_OUTER, K_INNER>(gx, TilePart{dx_part, d4, v0 > 0}, p.dx_cut, T_, s);
                 LAUNCH_CHECK("ce_dx");
+                // (a shorter last piece may make fewer; the others' sums stay)
+                if (v0 == 0 && made != p.dx_cut.parts) return fail(WINO_ERR_HIP, "dx: %d parts for %d", made, p.dx_cut.parts);
             }
             if (dw) {
                 if (p.dw_cut.parts == 1) {
                     tile_launch<T, K_OUTER, K_OUTER>(gw, dw_store, p.dw_cut, n, s);
                 } else {
-                    tile_launch<T, K_OUTER, K_OUTER>(gw, TilePart{dw_part, d4, 0}, p.dw_cut, n, s);
+                    const int made = tile_launch<T, K_OUTER, K_OUTER>(gw, TilePart{dw_part, d4, 0}, p.dw_cut, n, s);
                     LAUNCH_CHECK("ce_dw");
+                    if (made != p.dw_cut.parts) return fail(WINO_ERR_HIP, "dw: %d parts for %d", made, p.dw_cut.parts);
                     hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(D, 4) * n, 256)), dim3(256), 0, s,
                                        dw_part, p.dw_cut.parts, d4, D, n, dw_store);
                 }

@@ -112,8 +112,9 @@ int product(unsigned flags, int M, int N, int K, const void* xc, const void* xs,
     const size_t need = part_bytes(N, M, pick.parts);
     if (!work || work_bytes < need) return fail(WINO_ERR_WORKSPACE, "mx4 product: workspace of %zu bytes, %zu needed", work ? work_bytes : 0, need);
     const long pitch = round_up(N, 4);
-    tile_launch<mx4_t, K_INNER, K_INNER>(g, TilePart{static_cast<float*>(work), pitch, 0}, pick, M, s);
+    const int made = tile_launch<mx4_t, K_INNER, K_INNER>(g, TilePart{static_cast<float*>(work), pitch, 0}, pick, M, s);
     LAUNCH_CHECK("mx4 product in parts");
+    if (made != pick.parts) return fail(WINO_ERR_HIP, "mx4 product: %d parts for %d", made, pick.parts);
     hipLaunchKernelGGL((tile_join_kernel<T>), dim3(ceil_div((long)ceil_div(N, 4) * M, 256)), dim3(256), 0, s,
                        static_cast<const float*>(work), pick.parts, pitch, N, M, store);
     LAUNCH_CHECK("mx4 join");

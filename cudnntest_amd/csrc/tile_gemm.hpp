@@ -601,9 +601,10 @@ template <typename T, int AO, int BO, int BM, int BN, int RB> inline int tile_pr
 }
 
 template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
-inline void tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hipStream_t s) {
+inline int tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hipStream_t s) {
     parts = tile_prepare<T, AO, BO, BM, BN, RB>(g, parts, cover);
     hipLaunchKernelGGL((tile_gemm_kernel<T, AO, BO, BM, BN, WM, WN, RB, RING, Epi>), dim3(tile_grid(g.mt, g.nt), parts), dim3(64 * WM * WN), 0, s, g, epi);
+    return parts;
 }
 
 template <typename T> constexpr int kStageOf = 8 * TileElem<T>::piece;     // elements of k in 128 bytes
@@ -656,9 +657,10 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
     return best;
 }
 
-// `cover`: rows of n that the epilogue has to reach (N or a little more)
+// `cover`: rows of n that the epilogue has to reach (N or a little more).  Returns the parts that were launched: those of
+// the cut if it was picked for this reduction.
 template <typename T, int AO, int BO, class Epi>
-inline void tile_launch(const TileArgs& g, const Epi& epi, const TilePick& pick, int cover, hipStream_t s) {
+inline int tile_launch(const TileArgs& g, const Epi& epi, const TilePick& pick, int cover, hipStream_t s) {
     constexpr int RB = std::is_same<T, mx4_t>::value ? 64 : 128;
     if (pick.rows == 256) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
     if (pick.rows == 64) return tile_launch_as<T, AO, BO, 64, 64, 2, 2, RB, kSmallRing<T>>(g, epi, pick.parts, cover, s);

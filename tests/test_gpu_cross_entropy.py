@@ -308,3 +308,15 @@ def test_what_ignored_rows_hold_reaches_nothing(T, D, V, dtype):
     assert torch.equal(loss, want[0]) and torch.equal(lse[~off], want[1][~off]) and bool(torch.isnan(lse[off]).all())
     for got, ref in zip(ops.linear_cross_entropy_backward(grad, x, w, target, lse, bias=b), want[2:]):
         assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,D,V", [(164, 211, 476), (66, 299, 664), (97, 64, 700), (33, 80, 1100), (129, 24, 3000), (200, 130, 2100), (65, 520, 66)])
+def test_gradients_in_parts_of_two_values(T, D, V, dtype):
+    """dl as two values, products in parts: sizes whose padded reductions have a stage more than twice the plain one's.
+    The workspace comes in holding NaNs, so a part that is added without having been written shows."""
+    x, w, target, b, grad = problem(T, D, V, dtype)
+    torch.cuda.synchronize()
+    trash = [torch.full((1 << k,), NAN, device="cuda") for k in range(16, 24)]
+    del trash                                              # back to the allocator, for the calls below
+    check(x, w, target, b, grad)
