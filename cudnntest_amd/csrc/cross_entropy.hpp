@@ -293,8 +293,11 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(CeParts<T> p, CeRows rows
 // sums.  Called by a whole workgroup; ex holds one float per wave.
 __device__ __forceinline__ float weight_top(const float* grad, const CeRows& rows, int T, float top, float* ex) {
     float mx = 0.f;
-    for (int t = threadIdx.x; t < T; t += blockDim.x)
-        if (rows.target[t] != rows.ignore) mx = fmaxf(mx, fabsf(grad[t]));
+#pragma unroll 8
+    for (int t = threadIdx.x; t < T; t += blockDim.x) {
+        const float a = fabsf(grad[t]);                                // (read whether it counts or not: no load waits for another)
+        mx = fmaxf(mx, rows.target[t] != rows.ignore ? a : 0.f);
+    }
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
     if ((threadIdx.x & 63) == 0) ex[threadIdx.x >> 6] = mx;
