@@ -641,7 +641,7 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
             const int split = ceil_div(stages, parts);
             if (ceil_div(stages, split) != parts) continue;
             const long items = tiles * parts;
-            if (parts > 1 && (items > 4L * cus || (size_t)parts * M * N * 4 > (64u << 20))) break;
+            if (parts > 1 && (items > (rows == 64 ? 8L : 4L) * cus || (size_t)parts * M * N * 4 > (64u << 20))) break;
             const double k = (double)split * kStageOf<T>;
             const double mul = (double)rows * cols * k / (rate * kind.factor);
             const double move = (double)(rows + cols) * split * 128 / bytes;
