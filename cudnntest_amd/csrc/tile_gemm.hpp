@@ -6,14 +6,15 @@
 // one row per k); the four products of a linear layer and its gradients need both.  Types: fp32, f16, bf16, and
 // microscaled 4-bit values (mx4_t, K_INNER only).
 //
-// All types share one shape in BYTES: a stage is 128 bytes of k per operand row (32 fp32, 64 16-bit, 256 4-bit
-// elements), and a 16-byte piece of a row is one multiply's share of a lane (v_mfma_f32_32x32x16_{f16,bf16},
-// v_mfma_scale_f32_32x32x64_f8f6f4, or four v_mfma_f32_32x32x2_f32).  Lane half lh takes the pieces 4*lh + j,
-// j = 0..3: the sum does not care which half takes which k as long as both operands agree, and this way the block
-// scales of a lane's four 4-bit pieces are the four bytes of one dword, picked by the instruction's byte selector.
+// All types share one shape in BYTES: a stage is RB = 128 bytes of k per operand row (32 fp32, 64 16-bit elements; 64 bytes =
+// 128 elements of 4-bit operands, as they are stored), and a 16-byte piece of a row is one multiply's share of a lane
+// (v_mfma_f32_32x32x16_{f16,bf16}, v_mfma_scale_f32_32x32x64_f8f6f4, or four v_mfma_f32_32x32x2_f32).  Of a row's 2 S pieces
+// lane half lh takes S*lh + j, j = 0 .. S - 1: the sum does not care which half takes which k as long as both operands agree,
+// and this way the block scales of a lane's 4-bit pieces are neighbouring bytes, read at once and picked by the instruction's
+// byte selector.
 //
 // Operands move HBM -> LDS by direct 16-byte loads into a ring of stages; rows past the end are clamped to the last
-// one (their results are never stored).  LDS holds K_INNER rows of 128 bytes with their pieces exchanged by the row's
+// one (their results are never stored).  LDS holds K_INNER rows of RB bytes with their pieces exchanged by the row's
 // low bits, so that the 16-byte reads of 32 rows spread over the banks; K_OUTER tiles keep the k rows, and 16-bit
 // fragments are read through the transposing LDS read (ds_read_b64_tr_b16: the 16 lanes of a group supply four k rows
 // of 16 elements and each receives one column), fp32 ones element by element.
@@ -61,7 +62,7 @@ struct TileArgs {
     int pass, tail_at;      // stages of a pass; the one of them that does not exist in full, or -1 (set by the launch)
 };
 
-// the j-th of a lane's four scale bytes: a compile-time operand of the instruction
+// J: which of a lane's scale bytes, a compile-time operand of the instruction
 template <typename T, int J> __device__ __forceinline__ void tile_mma(const uintx4& a, const uintx4& b, floatx16& c, unsigned sa, unsigned sb) {
     if constexpr (std::is_same<T, mx4_t>::value) {
         const intx8 a8 = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
@@ -98,7 +99,6 @@ template <typename T, int ORDER, int EXT, int WAVES, int RB> struct TileSide {
     static constexpr int kLoads = kBytes / 1024 / WAVES;               // 1 KB loads per wave and stage
     static constexpr int kRow = EXT * TileElem<T>::bytes;              // K_OUTER: bytes of a k row in LDS
     static constexpr bool kOuter = ORDER == K_OUTER;
-    static constexpr bool kMx4 = std::is_same<T, mx4_t>::value;
     static_assert(kBytes % (1024 * WAVES) == 0, "whole loads per wave");
 
     uint64_t base;            // of the stage to load next
@@ -321,8 +321,8 @@ __device__ __forceinline__ void tile_gemm(const TileArgs& g, const Epi& epi, int
     auto multiply = [&](int s, auto jc, auto tail) {
         constexpr int J = decltype(jc)::value;
         if constexpr (decltype(tail)::value && !MX4) {
-            // pieces past the end of the reduction (two passes: whole stages): zero wherever k is inner (they were read from elsewhere in the
-            // row).  A k-outer operand needs no mask beside a k-inner one; where both are k-outer, the rows past
+            // pieces past the end of the reduction (two passes: whole stages): zero wherever k is inner (they were read
+            // from elsewhere in the row).  A k-outer operand needs no mask beside a k-inner one; where both are k-outer, the rows past
             // the end exist and one of the two holds zeros in them.
             const bool in = (TWO && g.passes > 1) || STEPS * lh + J < (g.K - s * STAGE + TileElem<T>::piece - 1) / TileElem<T>::piece;
 #pragma unroll
