@@ -445,17 +445,20 @@ def mx4_geometry(rows, K):
 
 
 @functools.lru_cache(maxsize=4096)
-def _mx4_shapes(rows, K):
-    kb = mx4_geometry(rows, K)["Kp"] // 128
-    return (kb, rows, 64), (kb, (rows + 3) // 4 * 4, 4)
+def _mx4_sizes(rows, K):
+    """(bytes of codes, where the scales start behind them in one buffer, bytes of that buffer)."""
+    g = mx4_geometry(rows, K)
+    at = (g["code_bytes"] + 15) // 16 * 16
+    return g["code_bytes"], at, at + g["scale_bytes"]
 
 
 class Mx4:
     """A matrix [rows][K] in microscaled 4-bit floating point (what wino_mx4_quantize writes): `codes`
     uint8 [Kp/128][rows][64], two elements a byte, and `scales` uint8 [Kp/128][rows rounded up to 4][4],
-    one power-of-two exponent per 32 columns; Kp is K rounded up to 128."""
+    one power-of-two exponent per 32 columns; Kp is K rounded up to 128.  mx4_quantize makes them; the
+    constructor takes codes and scales that are already there."""
 
-    __slots__ = ("codes", "scales", "rows", "K")
+    __slots__ = ("_buf", "_codes", "_scales", "_pc", "_ps", "rows", "K", "device")
 
     def __init__(self, codes, scales, rows, K):
         want = mx4_geometry(rows, K)
@@ -464,37 +467,59 @@ class Mx4:
         if codes.numel() != want["code_bytes"] or scales.numel() != want["scale_bytes"]:
             raise ValueError(f"a {rows} x {K} matrix has {want['code_bytes']} bytes of codes and {want['scale_bytes']} of "
                              f"scales, got {codes.numel()} and {scales.numel()}")
-        self.codes, self.scales, self.rows, self.K = codes, scales, int(rows), int(K)
+        if codes.device != scales.device or not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError("codes and scales must be contiguous and on one device")
+        self._buf, self._codes, self._scales = None, codes, scales
+        self._pc, self._ps = codes.data_ptr(), scales.data_ptr()
+        self.rows, self.K, self.device = int(rows), int(K), codes.device
 
     @classmethod
     def _empty(cls, rows, K, device):
+        # one buffer for both: an allocation less, and the two views only when somebody asks for them
         q = cls.__new__(cls)
-        codes, scales = _mx4_shapes(rows, K)
-        q.codes = torch.empty(codes, dtype=torch.uint8, device=device)
-        q.scales = torch.empty(scales, dtype=torch.uint8, device=device)
-        q.rows, q.K = rows, K
+        _, at, nbytes = _mx4_sizes(rows, K)
+        q._buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        q._codes = q._scales = None
+        q._pc = q._buf.data_ptr()
+        q._ps = q._pc + at
+        q.rows, q.K, q.device = rows, K, device
         return q
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            self._codes = self._buf[:_mx4_sizes(self.rows, self.K)[0]].view(-1, self.rows, 64)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._scales = self._buf[_mx4_sizes(self.rows, self.K)[1]:].view(-1, (self.rows + 3) // 4 * 4, 4)
+        return self._scales
 
     @property
     def shape(self):
         return (self.rows, self.K)
 
-    @property
-    def device(self):
-        return self.codes.device
+
+def _on_gpu(q, device, what):
+    if q.device != device:
+        raise ValueError(f"{what} is on {q.device}, the first tensor on {device}")
+    if device.type != "cuda":
+        raise ValueError("tensor must live on the GPU")
 
 
 def mx4_quantize(x, out=None):
     """x [rows][K] in microscaled 4 bits; `out` an Mx4 of the same shape to write into.  Asynchronous."""
     rows, K = _matrix(x, "x")
-    dt, dev = _dt(x), x.device
-    px = _ptr(x)
+    dt, px, dev = _dt(x), _ptr(x), x.device
     if out is None:
         out = Mx4._empty(rows, K, dev)
-    elif out.shape != (rows, K):
-        raise ValueError(f"out holds {out.shape}, x is {(rows, K)}")
-    _call(dev, _lib.load().wino_mx4_quantize, "wino_mx4_quantize", dt, rows, K, px, _address(out.codes, dev, "codes"),
-          _address(out.scales, dev, "scales"))
+    else:
+        if out.shape != (rows, K):
+            raise ValueError(f"out holds {out.shape}, x is {(rows, K)}")
+        _on_gpu(out, dev, "out")
+    _call(dev, _lib.load().wino_mx4_quantize, "wino_mx4_quantize", dt, rows, K, px, out._pc, out._ps)
     return out
 
 
@@ -502,10 +527,10 @@ def mx4_dequantize(q, dtype=torch.float32, out=None):
     """The values that q's codes stand for, [rows][K] of `dtype`."""
     if dtype not in _DTYPES:
         raise TypeError(f"unsupported dtype {dtype}")
-    dev = q.codes.device
+    dev = q.device
+    _on_gpu(q, dev, "q")
     out = _out_as(out, (q.rows, q.K), dtype, dev)
-    _call(dev, _lib.load().wino_mx4_dequantize, "wino_mx4_dequantize", _DTYPES[dtype], q.rows, q.K, _ptr(q.codes),
-          _address(q.scales, dev, "scales"), _address(out, dev, "out"))
+    _call(dev, _lib.load().wino_mx4_dequantize, "wino_mx4_dequantize", _DTYPES[dtype], q.rows, q.K, q._pc, q._ps, _address(out, dev, "out"))
     return out
 
 
@@ -521,11 +546,11 @@ def mx4_gemm(x, w, bias=None, relu=False, dtype=torch.float32, out=None):
         raise TypeError(f"unsupported dtype {dtype}")
     if x.K != w.K:
         raise ValueError(f"x has {x.K} columns, w has {w.K}")
-    M, N, K, dev = x.rows, w.rows, w.K, x.codes.device
+    M, N, K, dev = x.rows, w.rows, w.K, x.device
+    _on_gpu(w, dev, "w")
     _check_row_bias(bias, N, dtype)
     out = _out_as(out, (M, N), dtype, dev)
-    args = (_ptr(x.codes), _address(x.scales, dev, "x.scales"), _address(w.codes, dev, "w.codes"), _address(w.scales, dev, "w.scales"),
-            _address(bias, dev, "bias"), _address(out, dev, "out"))
+    args = (x._pc, x._ps, w._pc, w._ps, _address(bias, dev, "bias"), _address(out, dev, "out"))
     nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev).data_ptr() if nbytes else None
     _call(dev, _lib.load().wino_mx4_gemm, "wino_mx4_gemm", _DTYPES[dtype], FLAG_RELU if relu else 0, M, N, K, *args,
@@ -541,9 +566,10 @@ def mx4_linear(x, w, bias=None, relu=False, out=None):
         raise ValueError(f"x has {K} columns, w has {w.K}")
     N, dt, dev = w.rows, _dt(x), x.device
     _check_row_bias(bias, N, x.dtype)
+    px = _ptr(x)
+    _on_gpu(w, dev, "w")
     out = _out_as(out, (M, N), x.dtype, dev)
-    args = (_ptr(x), _address(w.codes, dev, "w.codes"), _address(w.scales, dev, "w.scales"), _address(bias, dev, "bias"),
-            _address(out, dev, "out"))
+    args = (px, w._pc, w._ps, _address(bias, dev, "bias"), _address(out, dev, "out"))
     nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev).data_ptr() if nbytes else None
     _call(dev, _lib.load().wino_mx4_linear, "wino_mx4_linear", dt, FLAG_RELU if relu else 0, M, N, K, *args, work, nbytes)

@@ -105,6 +105,12 @@ def test_python_layer_refuses():
         ops.Mx4(q.codes, q.scales, 4, 257)
     with pytest.raises(TypeError):
         ops.Mx4(q.codes.to(torch.int16), q.scales, 4, 32)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.Mx4(torch.zeros(1, 4, 128, dtype=torch.uint8)[..., ::2], q.scales, 4, 32)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.mx4_dequantize(q)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.mx4_gemm(q, q)
     with pytest.raises(ValueError, match="columns"):
         ops.mx4_linear(torch.zeros(4, 33), q)
     with pytest.raises(TypeError, match="bias"):
