@@ -237,6 +237,7 @@ template <typename T> struct Call {
             TileArgs gw = {};
             gw.a = outer<T>(xw, p.pitch_x, T_);
             gw.b = outer<T>(dl, pitch, p.rows);
+            gw.b.pieces = width * (int)sizeof(T) / 16;     // of one value: the second pass starts `width` elements into the row
             gw.M = D;
             gw.N = n;
             gw.K = T_;
