@@ -540,6 +540,14 @@ def _mx4_workspace_bytes(M, N, K, device_index):
         return _lib.load().wino_mx4_workspace_bytes(M, N, K)
 
 
+def _workspace(nbytes, dev):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _address_of(t):
+    return None if t is None else t.data_ptr()
+
+
 def mx4_gemm(x, w, bias=None, relu=False, dtype=torch.float32, out=None):
     """y = relu?(x w^T + bias) of two Mx4 matrices [M][K] and [N][K]; y and bias of `dtype`.  Asynchronous."""
     if dtype not in _DTYPES:
@@ -552,9 +560,9 @@ def mx4_gemm(x, w, bias=None, relu=False, dtype=torch.float32, out=None):
     out = _out_as(out, (M, N), dtype, dev)
     args = (x._pc, x._ps, w._pc, w._ps, _address(bias, dev, "bias"), _address(out, dev, "out"))
     nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev).data_ptr() if nbytes else None
+    work = _workspace(nbytes, dev)                         # (held until the launches are queued)
     _call(dev, _lib.load().wino_mx4_gemm, "wino_mx4_gemm", _DTYPES[dtype], FLAG_RELU if relu else 0, M, N, K, *args,
-          work, nbytes)
+          _address_of(work), nbytes)
     return out
 
 
@@ -571,8 +579,9 @@ def mx4_linear(x, w, bias=None, relu=False, out=None):
     out = _out_as(out, (M, N), x.dtype, dev)
     args = (px, w._pc, w._ps, _address(bias, dev, "bias"), _address(out, dev, "out"))
     nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev).data_ptr() if nbytes else None
-    _call(dev, _lib.load().wino_mx4_linear, "wino_mx4_linear", dt, FLAG_RELU if relu else 0, M, N, K, *args, work, nbytes)
+    work = _workspace(nbytes, dev)                         # (held until the launches are queued)
+    _call(dev, _lib.load().wino_mx4_linear, "wino_mx4_linear", dt, FLAG_RELU if relu else 0, M, N, K, *args,
+          _address_of(work), nbytes)
     return out
 
 
