@@ -8,23 +8,25 @@
 // The products run on tile_gemm_kernel with the vocabulary on the tile's m side: a lane then holds one row t and up to
 // 64 of its logits in registers, so the softmax statistics of a tile need no exchange between lanes but one.
 // Forward: every tile leaves (max, sum of exp) per row, 8 bytes for 128 logits, and one kernel joins them.  Backward:
-// the vocabulary is taken in pieces; a piece's dl (in the tensors' type) goes to scratch and feeds the two products.
-// Rounding dl to 16 bits adds about as much error as rounding the gradients themselves.  Over many rows these average;
-// up to kTwinRows rows a gradient can hang on a few entries of dl, so dl is then kept as two 16-bit values, what the type
-// holds and what it leaves over, and the two products run over both (their reduction twice as long, in calls that are
-// bound by their weights' bytes).
+// the vocabulary is taken in pieces; a piece's dl goes to scratch and feeds the two products and dbias.  In fp32 it is kept
+// as it is; in 16 bits as two values, what the type holds and what that leaves over (16 bits of significand in bf16, 22 in
+// f16), and the products run over both, their reduction twice as long.  One value would not do, at any number of rows: its
+// rounding makes the gradients' error 1.3 to 1.4 of their own rounding where the terms of their sums do not cancel, and 4.4 of
+// it in dx where the classes' rows of w share a component five times as long as what tells them apart.  It would be a third
+// faster where the multiplies bound the call (2048 rows, 32000 classes, D = 2048 in bf16: 1010 us for 1500).
 //
-// What bounds it: the multiplies.  2048 rows, 32000 classes, D = 2048 in bf16: four products of 268 GFLOP each at 237 to
-// 258 us (1.04 to 1.13 PFLOP/s), 10 us for the statistics and the row weights, 19 us to join dx's parts.  In fp32 (777 x
-// 10007 x 1003) the matrix pipe is busy for 0.8 of the products' time.  Small problems are bound by their launches: 250 rows,
-// 1000 classes, D = 4096 in f16 take 46 us in five kernels, none above 23.
+// What bounds it: the multiplies.  That problem: the logits, twice, at 240 us and, with dl's two stores, 300 us; dx and dw
+// over two values 2 x 237 and 2 x 232 us in two pieces of the vocabulary (1.04 to 1.15 PFLOP/s); 10 us for the statistics and
+// the row weights, 13 us to join dx's parts.  In fp32 (777 x 10007 x 1003) the matrix pipe is busy for 0.8 of the products'
+// time.  Small problems are bound by their launches: 250 rows, 1000 classes, D = 4096 in f16 take 46 us in five kernels, none
+// above 23.
 #pragma once
 #include "common.hpp"
 #include "tile_gemm.hpp"
 
 namespace wino {
 
-constexpr int kTwinRows = 256;
+template <typename T> constexpr int kValues = sizeof(T) == 2 ? 2 : 1;  // that dl is kept as
 
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
@@ -153,8 +155,8 @@ template <typename T> struct CeDl {
     int v0;                 // first class of the piece
     T* dl;
     long pitch;             // elements from row to row
-    int width;              // of a row, a multiple of 8; twin: followed by `width` elements of what rounding left over
-    int row_end, twin;
+    int width;              // of a row, a multiple of 8; two values: followed by `width` elements of what rounding left over
+    int row_end;
     template <int BM, int BN, int WM, int WN, int MI, int NI>
     __device__ __forceinline__ void run(floatx16 (&acc)[MI][NI], const TileArgs& g, int m0, int n0, int wm, int wn, int l32, int lh, char* lds) const {
         const float f = scale ? *scale : 1.f;
@@ -175,26 +177,34 @@ template <typename T> struct CeDl {
             const int first = m0 + wm * MI * 32;
             none[n] = !__any(hit[n] >= first && hit[n] < first + MI * 32);
         }
-        auto value = [&](int i, int q, int n, float (&v)[4]) {
-            const int m = m0 + (wm * MI + i) * 32 + 8 * q + 4 * lh;
+        // logits to dl where they are, once for both stores
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
             const ExpFrom<T> p(z[n]);
             if (plain && none[n]) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = ignored[n] ? 0.f : p(acc[i][n][4 * q + e]) * weight[n];
-                return;
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][n][r] = ignored[n] ? 0.f : p(acc[i][n][r]) * weight[n];
+                continue;
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float b = bias && m + e < g.M ? to_f32(bias[m + e]) : 0.f;
-                v[e] = m + e < g.M ? dl_of(acc[i][n][4 * q + e] + b, p, hit[n] == m + e, weight[n], ignored[n]) : 0.f;
-            }
-        };
-        tile_store<T, WM, WN, MI, NI>(dl, pitch, m0, n0, row_end, width, wm, wn, l32, lh, lds, false, value);
-        if (twin)
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int m = m0 + (wm * MI + i) * 32 + 8 * (r >> 2) + 4 * lh + (r & 3);
+                    const float b = bias && m < g.M ? to_f32(bias[m]) : 0.f;
+                    acc[i][n][r] = m < g.M ? dl_of(acc[i][n][r] + b, p, hit[n] == m, weight[n], ignored[n]) : 0.f;
+                }
+        }
+        tile_store<T, WM, WN, MI, NI>(dl, pitch, m0, n0, row_end, width, wm, wn, l32, lh, lds, false, [&](int i, int q, int n, float (&v)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][n][4 * q + e];
+        });
+        if constexpr (kValues<T> == 2)
             tile_store<T, WM, WN, MI, NI>(dl + width, pitch, m0, n0, row_end, width, wm, wn, l32, lh, lds, false, [&](int i, int q, int n, float (&v)[4]) {
-                value(i, q, n, v);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = left_over<T>(v[e]);
+                for (int e = 0; e < 4; ++e) v[e] = left_over<T>(acc[i][n][4 * q + e]);
             });
     }
 };
@@ -382,7 +392,7 @@ __global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int
         v[e] = in && m + e < o.rows.V ? dl_of(l[e] + b, ExpFrom<T>(z), target == m + e, weight, ignored) : 0.f;
     }
     store4<T>(o.dl + (long)t * o.pitch + m, v, 4, true);
-    if (o.twin) {
+    if constexpr (kValues<T> == 2) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = left_over<T>(v[e]);
         store4<T>(o.dl + (long)t * o.pitch + o.width + m, v, 4, true);
@@ -393,14 +403,14 @@ __global__ __launch_bounds__(256) void ce_dl_kernel(CeParts<T> p, CeDl<T> o, int
 template <typename T> struct CeBias {
     const T* dl;
     long pitch;
-    int width, twin, rows, V;
+    int width, rows, V;
     const float* scale;
     T* dbias;
     __device__ __forceinline__ void run(int block, float* ex) const {  // ex [16][64]
         const int c = threadIdx.x & 63, v = block * 64 + c, waves = blockDim.x >> 6;
         for (int g = threadIdx.x >> 6; g < 16; g += waves) {
             float s = 0.f;
-            for (int two = 0; v < V && two <= twin; ++two) {
+            for (int two = 0; v < V && two < kValues<T>; ++two) {
                 const T* at = dl + two * width + v;
                 int t = g;
                 for (; t + 112 < rows; t += 128) {                     // eight loads in flight

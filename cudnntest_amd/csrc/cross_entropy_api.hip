@@ -11,7 +11,12 @@ bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p
 
 constexpr int kMaxCols = 1 << 21;                     // the kernels' 32-bit offsets inside a tile rest on it
 constexpr long kMaxTiles = 1L << 27;                  // of 128 x 128
-constexpr size_t kPieceBytes = 128u << 20;            // dl of one piece of the vocabulary: half of the last-level cache
+// dl of one piece of the vocabulary: half of the last-level cache (2048 x 32000 x 2048 bf16 with 64 / 128 / 256 MB: 1635 /
+// 1567 / 1566 us)
+constexpr size_t kPieceBytes = 128u << 20;
+// Rows of a backward call in 16 bits: dl of the smallest piece (128 classes, two values) is then 256 GB.  Twice as many are
+// the length of dw's reduction, an int.
+constexpr int kMaxTwinRows = 1 << 29;
 
 // Where everything is in the workspace, and how the problem is cut.  The same function sizes the workspace and drives
 // the calls.
@@ -22,7 +27,6 @@ struct Plan {
     TilePick logit, dx_cut, dw_cut;     // how the three products are cut
     int rows;                           // of dl: T rounded up to a stage
     int piece;                          // classes per piece (backward)
-    bool twin;                          // dl as two 16-bit values
     bool together;                      // dx, dw and dbias in one launch
     size_t x, w, logits, stats, picked, scale, dl, dx, dw, total;
 };
@@ -48,8 +52,7 @@ template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x
     p.pitch_w = p.pad_w ? padded : D;
     p.logit = tile_pick<E>(V, T, D, kMostParts, cus);
     p.rows = (int)round_up(T, 64);
-    p.twin = e == 2 && T <= kTwinRows;
-    const int two = p.twin ? 2 : 1;
+    constexpr int two = kValues<E>;
     p.small = p.logit.parts > 1 && (!backward || (size_t)p.rows * round_up(V, 128) * e * two <= kPieceBytes);
     size_t at = 0;
     if (p.pad_x || backward) p.x = place(at, (size_t)T * p.pitch_x * e);
@@ -68,8 +71,8 @@ template <typename E> Plan plan_as(int dtype, int T, int D, int V, const void* x
         p.dl = place(at, (size_t)p.rows * round_up(p.piece, 128) * e * two);
         if (!p.small) p.logit = tile_pick<E>(p.piece, T, D, 1, cus);
         // the reductions as they run: twice over whole stages where dl is two values (the join adds as many parts as the cut has)
-        p.dx_cut = tile_pick<E>(D, T, p.twin ? 2 * (int)round_up(p.piece, kStageOf<E>) : p.piece, kMostParts, cus);
-        p.dw_cut = tile_pick<E>(D, p.piece, p.twin ? 2 * p.rows : T, kMostParts, cus);
+        p.dx_cut = tile_pick<E>(D, T, two > 1 ? two * (int)round_up(p.piece, kStageOf<E>) : p.piece, kMostParts, cus);
+        p.dw_cut = tile_pick<E>(D, p.piece, two > 1 ? two * p.rows : T, kMostParts, cus);
         // one launch for the gradients while 64 x 64 tiles of both are a few to a CU, and whole sums are the better cut
         p.together = p.piece == V && p.dx_cut.parts == 1 && p.dw_cut.parts == 1 &&
                      (long)ceil_div(D, 64) * (ceil_div(T, 64) + ceil_div(V, 64)) <= kTogetherTiles * (long)cus;
@@ -96,6 +99,11 @@ int check(const char* what, int dtype, int T, int D, int V, const void* x, const
     const size_t e = dtype_size(dtype);
     if (misaligned(x, e) || misaligned(w, e) || (bias && misaligned(bias, e)) || misaligned(target, 8))
         return fail(WINO_ERR_INVALID, "%s: tensors must be aligned to their element type", what);
+    return WINO_OK;
+}
+
+int check_backward(const char* what, int dtype, int T) {
+    if (dtype != WINO_F32 && T > kMaxTwinRows) return fail(WINO_ERR_UNSUPPORTED, "%s: T = %d, at most %d in 16 bits", what, T, kMaxTwinRows);
     return WINO_OK;
 }
 
@@ -208,8 +216,8 @@ template <typename T> struct Call {
         for (int v0 = 0; v0 < V; v0 += p.piece) {
             const int n = std::min(p.piece, V - v0);
             const int width = (int)round_up(n, 128);
-            const long pitch = p.twin ? 2L * width : width;
-            const CeDl<T> out = {bias ? bias + v0 : nullptr, rows, lse, grad, scale_inside ? nullptr : scale, v0, dl, pitch, width, p.rows, p.twin};
+            const long pitch = (long)kValues<T> * width;
+            const CeDl<T> out = {bias ? bias + v0 : nullptr, rows, lse, grad, scale_inside ? nullptr : scale, v0, dl, pitch, width, p.rows};
             if (p.small) {
                 CeParts<T> parts;
                 if ((rc = partial_logits(&parts))) return rc;
@@ -227,7 +235,7 @@ template <typename T> struct Call {
             gx.M = D;
             gx.N = T_;
             gx.K = n;
-            if (p.twin) {               // over dl, then over what it leaves; w from its start again
+            if (kValues<T> == 2) {      // over dl, then over what it leaves; w from its start again
                 gx.K = (int)round_up(n, kStageOf<T>);
                 gx.passes = 2;
                 gx.a_turn = -(long)gx.K * gx.a.pitch;
@@ -241,14 +249,14 @@ template <typename T> struct Call {
             gw.M = D;
             gw.N = n;
             gw.K = T_;
-            if (p.twin) {
+            if (kValues<T> == 2) {
                 gw.K = p.rows;
                 gw.passes = 2;
                 gw.a_turn = -(long)gw.K * gw.a.pitch;
                 gw.b_turn = -(long)gw.K * gw.b.pitch + width * (long)sizeof(T);
             }
             const TileStore<T> dw_store = {dw ? dw + (long)v0 * D : nullptr, D, nullptr, back, 0};
-            const CeBias<T> bias_sum = {dl, pitch, width, p.twin, T_, n, back, dbias ? dbias + v0 : nullptr};
+            const CeBias<T> bias_sum = {dl, pitch, width, T_, n, back, dbias ? dbias + v0 : nullptr};
             if (p.together && dx && dw) {
                 tile_prepare<T, K_OUTER, K_INNER, 64, 64, 128>(gx, 1, T_);
                 tile_prepare<T, K_OUTER, K_OUTER, 64, 64, 128>(gw, 1, n);
@@ -312,6 +320,7 @@ extern "C" {
 size_t wino_linear_cross_entropy_workspace_bytes(int dtype, int T, int D, int V, const void* x, const void* w, int backward) {
     static const long long any = 0;
     if (check("wino_linear_cross_entropy_workspace_bytes", dtype, T, D, V, x, w, nullptr, &any)) return 0;
+    if (backward && check_backward("wino_linear_cross_entropy_workspace_bytes", dtype, T)) return 0;
     return plan(dtype, T, D, V, x, w, backward != 0).total;
 }
 
@@ -332,6 +341,7 @@ int wino_linear_cross_entropy_backward(int dtype, int T, int D, int V, const voi
                                        const long long* target, long long ignore_index, const float* grad, const float* lse, void* dx,
                                        void* dw, void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
     int rc = check("wino_linear_cross_entropy_backward", dtype, T, D, V, x, w, bias, target);
+    if (!rc) rc = check_backward("wino_linear_cross_entropy_backward", dtype, T);
     if (rc) return rc;
     if (!grad || !lse) return fail(WINO_ERR_INVALID, "wino_linear_cross_entropy_backward: null grad or lse");
     if (!dx && !dw && !dbias) return fail(WINO_ERR_INVALID, "wino_linear_cross_entropy_backward: no gradient asked for");

@@ -364,8 +364,8 @@ int wino_linear_cross_entropy(int dtype, int T, int D, int V, const void *x, con
  * [v == target[t]]) (zeros for an ignored row, NaN for a row with an invalid target)
  *     dx = dl w,   dw = dl^T x,   dbias[v] = sum_t dl[t][v]
  * in `dtype`; any of the three may be NULL.  The logits are computed again, a piece of the vocabulary at a time; dl
- * enters the products in `dtype`, relative to the largest weight (for 256 rows and fewer as two such values, so that no
- * rounding of dl shows in the gradients); sums are fp32. */
+ * enters the products relative to the largest weight, in fp32 as it is, in 16 bits as two values of `dtype`, so that no
+ * rounding of dl shows in the gradients (up to 2^29 rows); sums are fp32. */
 int wino_linear_cross_entropy_backward(int dtype, int T, int D, int V, const void *x, const void *w, const void *bias,
                                        const long long *target, long long ignore_index, const float *grad, const float *lse,
                                        void *dx, void *dw, void *dbias, void *workspace, size_t workspace_bytes, void *stream);

@@ -1,10 +1,11 @@
-"""Calls of the head that a program makes around the plain ones: several threads on one stream."""
+"""Calls of the head that a program makes around the plain ones: several threads on one stream, gradients whose terms cancel."""
 import threading
 
 import pytest
 import torch
 
 from cudnntest_amd import ops
+from head_reference import E32, Ce
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -36,3 +37,49 @@ def test_two_threads_on_one_stream():
     for k in range(2):
         assert len(got[k]) == 40
         assert all(torch.equal(y, ref) for ys in got[k] for y, ref in zip(ys, want[k]))
+
+
+def gradients_and_reference(T, D, V, dtype, keep=None, common=0.0, std=1.5):
+    """`common`: a component that all classes' weights share, in units of their own; `keep`: rows that are not ignored."""
+    x = rand((T, D), dtype, T + D)
+    w = ((rand((V, D), torch.float32, V + D) + common * rand((1, D), torch.float32, V)) * std / D ** 0.5).to(dtype)
+    b = rand((V,), dtype, V, 0.5)
+    target = torch.randint(0, V, (T,), generator=torch.Generator(device="cuda").manual_seed(T), device="cuda")
+    if keep is not None:
+        target[keep:] = -100
+    grad = (torch.rand(T, generator=torch.Generator(device="cuda").manual_seed(V), device="cuda") + 0.5) / T
+    loss, lse = ops.linear_cross_entropy(x, w, target, bias=b)
+    got = ops.linear_cross_entropy_backward(grad, x, w, target, lse, bias=b)
+    return got, Ce(x, w, target, b, -100, grad), (x, w, b, target, grad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,D,V,keep,common,std", [
+    (300, 64, 10, None, 0.0, 0.1),                         # few classes: dbias is a difference of sums that nearly cancel
+    (1000, 64, 10, None, 0.0, 0.1),
+    (2048, 40, 300, 4, 0.0, 1.5),                          # a padded batch with four rows that count
+    (300, 64, 1000, 3, 0.0, 1.5),
+    (1000, 64, 1000, None, 5.0, 1.5),                      # classes that share a component, which dx cancels
+    (700, 64, 9000, None, 5.0, 1.5),
+    (257, 72, 33, None, 0.0, 1.5),
+    (2048, 64, 20000, None, 0.0, 1.5)])                    # several pieces of the vocabulary
+def test_gradients_carry_no_rounding_of_dl(T, D, V, keep, common, std, dtype):
+    """At any number of rows the gradients' error is that of their own rounding, also where the sums over dl cancel.
+
+    dl as two values of the type is off by 2^-17 (bf16) or 2^-22 (f16) of itself; its probabilities carry the fp32 noise of
+    their logits, D roundings of random sign of at most 2^-24 of the largest logit, and four more of the bias, the statistics
+    and the exponent.  That error r relative to dl reaches a gradient as at most r times the sum of its terms' magnitudes."""
+    got, ref, (x, w, b, target, grad) = gradients_and_reference(T, D, V, dtype, keep, common, std)
+    X, W = x.double(), w.double()
+    l = X @ W.t().contiguous() + b.double()
+    g = torch.where(target != -100, grad.double(), torch.zeros_like(ref.lse))
+    p = (l - ref.lse.unsqueeze(1)).exp()
+    rows = torch.arange(T, device="cuda")[target != -100]
+    p[rows, target[rows]] -= 1.0
+    d = (p * g.unsqueeze(1)).abs()
+    r = {torch.float16: 2.0 ** -22, torch.bfloat16: 2.0 ** -17}[dtype] + E32 * ((D ** 0.5 + 4) * l.abs().max() + 8)
+    terms = (d @ W.abs(), d.t().contiguous() @ X.abs(), d.sum(0))
+    for name, a, want, mag in zip(("dx", "dw", "dbias"), got, (ref.dx, ref.dw, ref.db), terms):
+        best = (want.to(dtype).double() - want).norm()     # rounded once
+        err = (a.double() - want).norm()
+        assert err <= 1.05 * best + r * mag.norm(), f"{name}: {(err / best).item():.2f} of one rounding"

@@ -1,11 +1,12 @@
 """How long the head's Python calls keep what they hand to the library, on the CPU: a workspace that is back with the
 allocator before its launches are queued can be handed to another thread's call on the same stream."""
+import ctypes
 import weakref
 
 import pytest
 import torch
 
-from cudnntest_amd import ops
+from cudnntest_amd import _lib, ops
 
 BYTES = 12345
 
@@ -43,3 +44,15 @@ def test_workspace_lives_until_the_call_has_returned(name, monkeypatch):
     monkeypatch.setattr(ops, "_ce_workspace_bytes", lambda *a: BYTES)
     calls()[name]()
     assert seen == [True]
+
+
+def test_more_rows_than_a_reduction_counts_are_refused():
+    """dw of 16-bit tensors reduces over two values a row: past 2^29 rows (256 GB of dl) the call is refused, not cut short."""
+    L, P = _lib.load(), ctypes.c_void_p(256)
+    size = lambda dt, T, backward: L.wino_linear_cross_entropy_workspace_bytes(dt, T, 1, 100, P, P, backward)
+    for dt in (1, 2):
+        assert size(dt, 1 << 29, 1) >= (1 << 29) * 128 * 2 * 2 and size(dt, (1 << 29) + 1, 1) == 0
+        assert size(dt, (1 << 29) + 1, 0) > 0
+        rc = L.wino_linear_cross_entropy_backward(dt, (1 << 29) + 1, 1, 100, P, P, None, P, -100, P, P, P, P, None, P, 1 << 60, None)
+        assert rc == -2 and b"at most" in L.wino_last_error()
+    assert size(0, (1 << 29) + 1, 1) > 0
