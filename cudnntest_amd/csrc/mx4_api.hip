@@ -9,6 +9,11 @@ namespace {
 bool valid_dtype(int d) { return d == WINO_F32 || d == WINO_F16 || d == WINO_BF16; }
 bool misaligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    return p < q + nb && q < p + na;
+}
+
 // limits that the kernels' 32-bit offsets inside a tile rest on
 constexpr int kMaxCols = 1 << 21;
 constexpr long kMaxTiles = 1L << 27;            // of 128 x 128
@@ -200,6 +205,10 @@ int wino_mx4_linear(int dtype, unsigned flags, int M, int N, int K, const void* 
     if (rc) return rc;
     if (!x) return fail(WINO_ERR_INVALID, "wino_mx4_linear: null input");
     if (misaligned(x, dtype_size(dtype))) return fail(WINO_ERR_INVALID, "wino_mx4_linear: x must be aligned to its element type");
+    // this kernel's workgroups all read x, and store their columns of y when they are done: one may still read what another
+    // has written over
+    if (few_quant(M, K) && overlap(x, (size_t)M * K * dtype_size(dtype), y, (size_t)M * N * dtype_size(dtype)))
+        return fail(WINO_ERR_INVALID, "wino_mx4_linear: y must not overlap x in a call without a workspace (quantise x first)");
     if (few_quant(M, K)) return few_rows_any(dtype, flags, M, N, K, x, nullptr, nullptr, wcodes, wscales, bias, y, (hipStream_t)stream);
     const size_t need = wino_mx4_workspace_bytes(M, N, K);
     if (!workspace || workspace_bytes < need)

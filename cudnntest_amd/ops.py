@@ -568,7 +568,8 @@ def mx4_gemm(x, w, bias=None, relu=False, dtype=torch.float32, out=None):
 
 def mx4_linear(x, w, bias=None, relu=False, out=None):
     """y = relu?(x w^T + bias): a fully connected layer with 4-bit weights w (Mx4 [N][K]) on x [M][K], which is
-    quantised on the way in: the bits of mx4_gemm(mx4_quantize(x), w, bias, relu, x.dtype).  Asynchronous."""
+    quantised on the way in: the bits of mx4_gemm(mx4_quantize(x), w, bias, relu, x.dtype).  `out` may lie over x.
+    Asynchronous."""
     M, K = _matrix(x, "x")
     if K != w.K:
         raise ValueError(f"x has {K} columns, w has {w.K}")
@@ -576,9 +577,12 @@ def mx4_linear(x, w, bias=None, relu=False, out=None):
     _check_row_bias(bias, N, x.dtype)
     px = _ptr(x)
     _on_gpu(w, dev, "w")
-    out = _out_as(out, (M, N), x.dtype, dev)
-    args = (px, w._pc, w._ps, _address(bias, dev, "bias"), _address(out, dev, "out"))
+    given, out = out, _out_as(out, (M, N), x.dtype, dev)
+    py = _address(out, dev, "out")
     nbytes = _mx4_workspace_bytes(M, N, K, dev.index)
+    if given is not None and not nbytes and px < py + M * N * x.element_size() and py < px + M * K * x.element_size():
+        return mx4_gemm(mx4_quantize(x), w, bias, relu, x.dtype, out)      # the kernel without a workspace reads x to its end
+    args = (px, w._pc, w._ps, _address(bias, dev, "bias"), py)
     work = _workspace(nbytes, dev)                         # (held until the launches are queued)
     _call(dev, _lib.load().wino_mx4_linear, "wino_mx4_linear", dt, FLAG_RELU if relu else 0, M, N, K, *args,
           _address_of(work), nbytes)

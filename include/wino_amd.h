@@ -320,7 +320,7 @@ int wino_stack_destroy(wino_stack_t *stack);
  * microscaled 4-bit floating point, and the loss of the last layer with its gradient.  No counterpart in the reference.
  *
  * These calls use only the buffers they are given: calls on different streams may overlap if their workspaces and outputs
- * are different buffers.  They allocate nothing, never synchronise, record no memset and can be captured into a graph.
+ * are different buffers.  Outputs do not overlap inputs (but see wino_mx4_linear).  They allocate nothing, never synchronise, record no memset and can be captured into a graph.
  * Results do not depend on timing: sums that are cut are joined in a fixed order.  The device that owns the buffers must
  * be the current one.  Matrices are row-major and contiguous.
  *
@@ -343,7 +343,8 @@ size_t wino_mx4_workspace_bytes(int M, int N, int K);
  * fp32, y and bias (N elements or NULL) are of `dtype`.  flags: 0 or WINO_FLAG_RELU. */
 int wino_mx4_gemm(int dtype, unsigned flags, int M, int N, int K, const void *xcodes, const void *xscales, const void *wcodes,
                   const void *wscales, const void *bias, void *y, void *workspace, size_t workspace_bytes, void *stream);
-/* The same with x [M][K] given in `dtype` and quantised on the way in: the bits of wino_mx4_quantize + wino_mx4_gemm. */
+/* The same with x [M][K] given in `dtype` and quantised on the way in: the bits of wino_mx4_quantize + wino_mx4_gemm.  y may
+ * lie over x where the call needs a workspace; without one x is read while y is written, and an overlap is refused. */
 int wino_mx4_linear(int dtype, unsigned flags, int M, int N, int K, const void *x, const void *wcodes, const void *wscales,
                     const void *bias, void *y, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -1,4 +1,5 @@
-"""Calls of the head that a program makes around the plain ones: several threads on one stream, gradients whose terms cancel."""
+"""Calls of the head that a program makes around the plain ones: several threads on one stream, an output over its input,
+gradients whose terms cancel."""
 import threading
 
 import pytest
@@ -83,3 +84,18 @@ def test_gradients_carry_no_rounding_of_dl(T, D, V, keep, common, std, dtype):
         best = (want.to(dtype).double() - want).norm()     # rounded once
         err = (a.double() - want).norm()
         assert err <= 1.05 * best + r * mag.norm(), f"{name}: {(err / best).item():.2f} of one rounding"
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,N", [(1, 4096), (3, 256), (8, 4096), (16, 1024), (20, 1024), (40, 512), (300, 1000)])
+def test_layer_in_place(M, N, dtype):
+    """`out` over x, exactly or in part: the bits of a separate output."""
+    w, b = ops.mx4_quantize(rand((N, N), dtype, N, 0.05)), rand((N,), dtype, 5)
+    x = rand((M, N), dtype, M)
+    want = ops.mx4_linear(x, w, bias=b, relu=True)
+    for off in (0, N, M * N // 2):
+        buf = torch.zeros(2 * M * N, dtype=dtype, device="cuda")
+        buf[:M * N] = x.view(-1)
+        out = buf[off:off + M * N].view(M, N)
+        y = ops.mx4_linear(buf[:M * N].view(M, N), w, bias=b, relu=True, out=out)
+        assert y.data_ptr() == out.data_ptr() and torch.equal(y, want)

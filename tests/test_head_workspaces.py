@@ -56,3 +56,15 @@ def test_more_rows_than_a_reduction_counts_are_refused():
         rc = L.wino_linear_cross_entropy_backward(dt, (1 << 29) + 1, 1, 100, P, P, None, P, -100, P, P, P, P, None, P, 1 << 60, None)
         assert rc == -2 and b"at most" in L.wino_last_error()
     assert size(0, (1 << 29) + 1, 1) > 0
+
+
+@pytest.mark.parametrize("dt,e", [(0, 4), (1, 2), (2, 2)])
+def test_output_over_the_input_of_few_rows_is_refused(dt, e):
+    """One launch quantises x and writes y: every workgroup reads all of x, so y must not lie over it."""
+    L, at = _lib.load(), 1 << 20
+    linear = lambda M, N, K, y: L.wino_mx4_linear(dt, 0, M, N, K, ctypes.c_void_p(at), ctypes.c_void_p(1 << 30), ctypes.c_void_p(1 << 29), None,
+                                                  ctypes.c_void_p(y), None, 0, None)
+    M, N, K = 4, 512, 1024
+    assert L.wino_mx4_workspace_bytes(M, N, K) == 0
+    for y in (at, at + 64, at + M * K * e - e, at - M * N * e + e):
+        assert linear(M, N, K, y) == -1 and b"overlap" in L.wino_last_error()
