@@ -306,15 +306,15 @@ __device__ __forceinline__ float weight_top(const float* grad, const CeRows& row
 #pragma unroll 8
     for (int t = threadIdx.x; t < T; t += blockDim.x) {
         const float a = fabsf(grad[t]);                                // (read whether it counts or not: no load waits for another)
-        mx = fmaxf(mx, rows.target[t] != rows.ignore ? a : 0.f);
+        // an infinite weight spoils its row of dx and all of dw, not the scale of the other rows of dx
+        mx = fmaxf(mx, rows.target[t] != rows.ignore && a <= 3.4028235e38f ? a : 0.f);
     }
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
     if ((threadIdx.x & 63) == 0) ex[threadIdx.x >> 6] = mx;
     __syncthreads();
     for (int w = 0; w < (int)(blockDim.x >> 6); ++w) mx = fmaxf(mx, ex[w]);
-    // no weight at all, or none that is finite: factor 1
-    return mx > 0.f && mx <= 3.4028235e38f ? fmaxf(mx, 1e-30f) : top;
+    return mx > 0.f ? fmaxf(mx, 1e-30f) : top;                         // no weight at all: factor 1
 }
 // out[0] = the factor, out[1] = its inverse
 __global__ __launch_bounds__(1024) static void ce_scale_kernel(const float* __restrict__ grad, CeRows rows, int T, float top, float* __restrict__ out) {

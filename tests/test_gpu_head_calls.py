@@ -99,3 +99,24 @@ def test_layer_in_place(M, N, dtype):
         out = buf[off:off + M * N].view(M, N)
         y = ops.mx4_linear(buf[:M * N].view(M, N), w, bias=b, relu=True, out=out)
         assert y.data_ptr() == out.data_ptr() and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,V", [(40, 300), (600, 9000), (1500, 300)])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_row_weight_that_is_not_finite_stays_in_its_row(T, V, bad, dtype):
+    """The loss of one row overflowed: the other rows of dx are those of a finite weight, bit for bit (it was not the largest,
+    so nothing else changes)."""
+    D = 64
+    x, w = rand((T, D), dtype, 1), rand((V, D), dtype, 2, 0.2)
+    target = torch.randint(0, V, (T,), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    target[::9] = -100
+    grad = (torch.rand(T, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda") + 0.5) / T
+    grad[5] = 0.25 / T
+    _, lse = ops.linear_cross_entropy(x, w, target)
+    want = ops.linear_cross_entropy_backward(grad, x, w, target, lse)[0]
+    grad[5] = bad
+    dx, dw, _ = ops.linear_cross_entropy_backward(grad, x, w, target, lse)
+    rest = torch.arange(T, device="cuda") != 5
+    assert torch.equal(dx[rest], want[rest]) and bool(torch.isfinite(want.float()).all())
+    assert not bool(torch.isfinite(dx[5].float()).any()) and not bool(torch.isfinite(dw.float()).any())
