@@ -421,7 +421,14 @@ def _call(device, fn, name, *args):
 def _matrix(t, what):
     if t.dim() != 2:
         raise ValueError(f"{what} must be a matrix, got {t.dim()} dimensions")
-    return t.shape
+    return _ints(t.shape, what)
+
+
+def _ints(sizes, what):
+    # (the library's sizes are C ints, and ctypes would pass on the low 32 bits of a larger one)
+    if max(sizes) > 0x7fffffff:
+        raise ValueError(f"{what}: sizes {tuple(sizes)} do not fit 32 bits")
+    return sizes
 
 
 def _out_as(out, shape, dtype, device):
@@ -439,6 +446,7 @@ def _check_row_bias(bias, n, dtype):
 
 def mx4_geometry(rows, K):
     import ctypes
+    _ints((rows, K), "matrix")
     kp, cb, sb = ctypes.c_int(), ctypes.c_size_t(), ctypes.c_size_t()
     _lib.check(_lib.load().wino_mx4_geometry(rows, K, kp, cb, sb), "wino_mx4_geometry")
     return dict(Kp=kp.value, code_bytes=cb.value, scale_bytes=sb.value)

@@ -68,3 +68,17 @@ def test_output_over_the_input_of_few_rows_is_refused(dt, e):
     assert L.wino_mx4_workspace_bytes(M, N, K) == 0
     for y in (at, at + 64, at + M * K * e - e, at - M * N * e + e):
         assert linear(M, N, K, y) == -1 and b"overlap" in L.wino_last_error()
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The C calls take int: a size past it must not arrive as its low 32 bits."""
+    long = torch.empty((1 << 32) + 5, 1, device="meta")
+    t, w = torch.zeros(5, dtype=torch.int64), torch.zeros(3, 1)
+    q = ops.Mx4(torch.zeros(64, dtype=torch.uint8), torch.zeros(16, dtype=torch.uint8), 1, 1)
+    f = torch.zeros(5)
+    for call in (lambda: ops.mx4_quantize(long), lambda: ops.mx4_linear(long, q), lambda: ops.linear_cross_entropy(long, w, t),
+                 lambda: ops.linear_cross_entropy(torch.zeros(5, 1), long, t), lambda: ops.linear_cross_entropy_backward(f, long, w, t, f),
+                 lambda: ops.mx4_geometry((1 << 32) + 5, 1), lambda: ops.mx4_geometry(5, (1 << 32) + 1),
+                 lambda: ops.Mx4(q.codes, q.scales, (1 << 32) + 1, 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
