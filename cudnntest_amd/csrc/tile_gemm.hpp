@@ -45,7 +45,7 @@ template <> struct TileElem<mx4_t> { static constexpr int piece = 32, bytes = 0;
 
 struct TileOperand {
     const char* p;          // first byte of the operand
-    const char* scale;      // mx4: [k stage][rows rounded up to 2][8] scale bytes
+    const char* scale;      // mx4: [k stage][rows rounded up to 4][4] scale bytes
     long pitch;             // K_INNER: bytes from row to row; K_OUTER: bytes from one k row to the next
     long step;              // bytes from stage to stage (set by the launch)
     int rows;               // K_INNER: rows (m or n); K_OUTER: k rows that may be read
@@ -310,7 +310,8 @@ __device__ __forceinline__ void tile_gemm(const TileArgs& g, const Epi& epi, int
     };
     auto read_scales = [&](int slot, int set) {
         if constexpr (MX4) {
-            typedef std::conditional_t<STEPS == 4, unsigned, unsigned short> SW;       // a lane's scale bytes of a stage
+            typedef unsigned short SW;                                 // a lane's scale bytes of a stage
+            static_assert(STEPS == (int)sizeof(SW), "a scale byte per step");
             const char* sca = lds + slot * SLOT + SA::kBytes + SB::kBytes;
 #pragma unroll
             for (int i = 0; i < MI; ++i) qa[set][i] = *reinterpret_cast<const SW*>(sca + ((wm * MI + i) * 32 + l32) * SROW + lh * STEPS);
@@ -583,6 +584,12 @@ constexpr int kTile = 128;               // edge of the usual tile
 
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
+// the parts that are not empty when `stages` are cut into `parts`
+inline int parts_of(int stages, int parts) { return ceil_div(stages, ceil_div(stages, parts)); }
+
+template <typename T> constexpr int kStageBytes = std::is_same<T, mx4_t>::value ? 64 : 128;   // of an operand row
+template <typename T> constexpr int kStageOf = kStageBytes<T> / 16 * TileElem<T>::piece;      // elements of k
+
 // the fields of g that follow from the tile and the parts; returns the parts that are not empty
 template <typename T, int AO, int BO, int BM, int BN, int RB> inline int tile_prepare(TileArgs& g, int parts, int cover) {
     g.mt = ceil_div(g.M, BM);
@@ -597,7 +604,7 @@ template <typename T, int AO, int BO, int BM, int BN, int RB> inline int tile_pr
     g.tail_at = g.passes > 1 ? (AO == K_OUTER && g.a.rows < g.K ? g.pass - 1 : -1) : g.K % stage ? g.pass - 1 : -1;
     g.stages = g.passes * g.pass;
     g.split = ceil_div(g.stages, parts);
-    return ceil_div(g.stages, g.split);
+    return parts_of(g.stages, parts);
 }
 
 template <typename T, int AO, int BO, int BM, int BN, int WM, int WN, int RB, int RING, class Epi>
@@ -606,8 +613,6 @@ inline int tile_launch_as(TileArgs g, const Epi& epi, int parts, int cover, hipS
     hipLaunchKernelGGL((tile_gemm_kernel<T, AO, BO, BM, BN, WM, WN, RB, RING, Epi>), dim3(tile_grid(g.mt, g.nt), parts), dim3(64 * WM * WN), 0, s, g, epi);
     return parts;
 }
-
-template <typename T> constexpr int kStageOf = 8 * TileElem<T>::piece;     // elements of k in 128 bytes
 
 // stages in LDS of a 64 x 64 tile: fp32 is bound by its multiplies and takes more workgroups to a CU instead
 template <typename T> constexpr int kSmallRing = std::is_same<T, mx4_t>::value ? 5 : sizeof(T) == 4 ? 2 : 3;
@@ -630,7 +635,9 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
     // relative to 128 x 128: the large tile draws half the bytes per product, the small ones more
     const struct { int rows, cols; double factor; } kinds[] = {
         {256, 256, F32 ? 1.0 : MX4 ? 1.23 : 1.33}, {kTile, kTile, 1.0}, {kTile, 64, F32 ? 0.9 : 0.8}, {kTile, 32, F32 ? 1.05 : 0.5}, {64, 64, F32 ? 1.0 : MX4 ? 0.8 : 0.6}};
-    const int stages = ceil_div(K, kStageOf<T>);
+    // the rates were fitted with cuts of 128 bytes of a row, two stages of 4-bit operands
+    constexpr int kUnit = 8 * TileElem<T>::piece;
+    const int stages = ceil_div(K, kUnit), launched = ceil_div(K, kStageOf<T>);
     TilePick best = {kTile, kTile, 1};
     double least = 1e30;
     for (const auto& kind : kinds) {
@@ -639,10 +646,10 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
         const long tiles = (long)ceil_div(M, rows) * ceil_div(N, cols);
         for (int parts = 1; parts <= most && parts <= std::max(1, stages / 2); parts += parts < 8 ? 1 : parts / 4) {
             const int split = ceil_div(stages, parts);
-            if (ceil_div(stages, split) != parts) continue;
+            if (parts_of(stages, parts) != parts || parts_of(launched, parts) != parts) continue;
             const long items = tiles * parts;
             if (parts > 1 && (items > (rows == 64 ? 8L : 4L) * cus || (size_t)parts * M * N * 4 > (64u << 20))) break;
-            const double k = (double)split * kStageOf<T>;
+            const double k = (double)split * kUnit;
             const double mul = (double)rows * cols * k / (rate * kind.factor);
             const double move = (double)(rows + cols) * split * 128 / bytes;
             // one small tile alone on its CU waits for its own loads
@@ -661,7 +668,7 @@ template <typename T> inline TilePick tile_pick(int M, int N, int K, int most, i
 // the cut if it was picked for this reduction.
 template <typename T, int AO, int BO, class Epi>
 inline int tile_launch(const TileArgs& g, const Epi& epi, const TilePick& pick, int cover, hipStream_t s) {
-    constexpr int RB = std::is_same<T, mx4_t>::value ? 64 : 128;
+    constexpr int RB = kStageBytes<T>;
     if (pick.rows == 256) return tile_launch_as<T, AO, BO, 256, 256, 2, 4, RB, RB == 64 ? 4 : 2>(g, epi, pick.parts, cover, s);
     if (pick.rows == 64) return tile_launch_as<T, AO, BO, 64, 64, 2, 2, RB, kSmallRing<T>>(g, epi, pick.parts, cover, s);
     if constexpr (RB == 128)            // (a 4-bit stage of 32 rows is less than a load per wave)
