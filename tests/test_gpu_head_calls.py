@@ -1,12 +1,12 @@
 """Calls of the head that a program makes around the plain ones: several threads on one stream, an output over its input,
-gradients whose terms cancel."""
+gradients whose terms cancel, long batches, graphs that share their memory."""
 import threading
 
 import pytest
 import torch
 
 from cudnntest_amd import ops
-from head_reference import E32, Ce
+from head_reference import E32, Ce, assert_within
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -120,3 +120,55 @@ def test_a_row_weight_that_is_not_finite_stays_in_its_row(T, V, bad, dtype):
     rest = torch.arange(T, device="cuda") != 5
     assert torch.equal(dx[rest], want[rest]) and bool(torch.isfinite(want.float()).all())
     assert not bool(torch.isfinite(dx[5].float()).any()) and not bool(torch.isfinite(dw.float()).any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,D,V", [(70001, 24, 40), (5000, 40, 1), (3001, 9000, 3), (20000, 130, 257), (257, 1, 128), (321, 4100, 129)])
+def test_many_rows(T, D, V, dtype):
+    """Long reductions of dw over two values a row, cut in parts or not, and the last stage of both passes ragged."""
+    x, w, b = rand((T, D), dtype, T), rand((V, D), dtype, V, 1.5 / D ** 0.5), rand((V,), dtype, D, 0.5)
+    target = torch.randint(0, V, (T,), generator=torch.Generator(device="cuda").manual_seed(T), device="cuda")
+    target[::11] = -100
+    grad = (torch.rand(T, generator=torch.Generator(device="cuda").manual_seed(V), device="cuda") + 0.5) / T
+    ref = Ce(x, w, target, b, -100, grad)
+    loss, lse = ops.linear_cross_entropy(x, w, target, bias=b)
+    assert_within(lse, ref.lse, ref.lse_tol, "lse")
+    assert_within(loss, ref.loss, ref.loss_tol, "loss")
+    got = ops.linear_cross_entropy_backward(grad, x, w, target, lse, bias=b)
+    for a, want, tol, name in zip(got, (ref.dx, ref.dw, ref.db), (ref.dx_tol, ref.dw_tol, ref.db_tol), ("dx", "dw", "dbias")):
+        assert_within(a, want, tol, name)
+    again = ops.linear_cross_entropy_backward(grad, x, w, target, lse, bias=b)
+    assert all(torch.equal(a, c) for a, c in zip(got, again))
+
+
+@pytest.mark.parametrize("T,V", [(300, 129), (600, 9000)])
+def test_two_graphs_of_one_pool_and_a_side_stream(T, V):
+    """Loss and gradients captured twice into graphs that share their memory, replayed in turn, and on a stream of its own."""
+    def problem(seed):
+        x, w = rand((T, 72), torch.bfloat16, seed), rand((V, 72), torch.bfloat16, seed + 1, 0.2)
+        return x, w, torch.randint(0, V, (T,), generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda"), rand((T,), torch.float32, seed + 2)
+
+    def step(x, w, target, grad):
+        loss, lse = ops.linear_cross_entropy(x, w, target)
+        return (loss, lse) + ops.linear_cross_entropy_backward(grad, x, w, target, lse)[:2]
+    jobs = [problem(10), problem(20)]
+    want = [step(*j) for j in jobs]
+    graphs, outs, pool = [], [], None
+    for j in jobs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(step(*j))
+        graphs.append(g)
+        pool = g.pool()
+    for _ in range(4):
+        for k in (0, 1):
+            graphs[k].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(outs[k], want[k]))
+            assert all(torch.equal(a, c) for a, c in zip(step(*jobs[k]), want[k]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(*jobs[0])
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, c) for a, c in zip(got, want[0]))
