@@ -16,9 +16,9 @@
 // faster where the multiplies bound the call (2048 rows, 32000 classes, D = 2048 in bf16: 1010 us for 1500).
 //
 // What bounds it: the multiplies.  That problem: the logits, twice, at 240 us and, with dl's two stores, 300 us; dx and dw
-// over two values 2 x 237 and 2 x 232 us in two pieces of the vocabulary (1.04 to 1.15 PFLOP/s); 10 us for the statistics and
+// over two values 2 x 237 and 2 x 232 us in two pieces of the vocabulary (1.13 to 1.15 PFLOP/s); 10 us for the statistics and
 // the row weights, 13 us to join dx's parts.  In fp32 (777 x 10007 x 1003) the matrix pipe is busy for 0.8 of the products'
-// time.  Small problems are bound by their launches: 250 rows, 1000 classes, D = 4096 in f16 take 46 us in five kernels, none
+// time.  Small problems are bound by their launches: 250 rows, 1000 classes, D = 4096 in f16 take 47 us in five kernels, none
 // above 23.
 #pragma once
 #include "common.hpp"
